@@ -130,6 +130,127 @@ int sched_paged_decode_append(const SchedDecodeArgs *a, const SchedKvAppendArgs 
 int sched_kv_table_update(int32_t *table, int64_t num_rows, int64_t width,
                           const int32_t *updates, uint32_t n, void *stream);
 
+/* ---- query / key norm and position rotation -------------------------------- */
+
+#define SCHED_ROTARY_ABI_VERSION 1u
+
+/* Per token i and head, over the head's d dims:
+ *   x' = x * weight / sqrt(mean(x^2) + eps)     (weight NULL: x' = x)
+ * then the rotation of the first rot_dim dims by the token's angles: with p =
+ * positions[i] and c_j = cos_sin[p][j], s_j = cos_sin[p][rot_dim/2 + j],
+ *   (y_a, y_b) = (x'_a c_j - x'_b s_j, x'_b c_j + x'_a s_j)
+ * for the pairs (a, b) = (j, j + rot_dim/2), or (2j, 2j+1) if interleaved. Dims past
+ * rot_dim pass through. All in fp32, rounded once at the end (to nearest even).
+ *
+ * Query rows go to q_out. Key rows go to k_out, or, with a cache (k_pool not
+ * NULL), into it together with the value rows, at the places of sched_kv_append's
+ * rule: token rows append_indptr[r] .. append_indptr[r+1]-1 are request r's, and land at
+ * ctx_lens[r] - n_r .. ctx_lens[r] - 1. The cache has the rows' dtype and token-major
+ * V. Outputs may be their inputs (in place); else they must not overlap.
+ *
+ * `errors` (NULL = none) counts tokens whose position lies outside [0, max_pos),
+ * none of whose rows is written, and (token, kv-head) pairs that have no place in the
+ * cache (as sched_kv_append's); their key and value rows are not written.
+ * Serves the model code right before the reference's decode; no counterpart in
+ * it. */
+typedef struct SchedRotaryArgs {
+  uint32_t abi_version;   /* SCHED_ROTARY_ABI_VERSION */
+  uint32_t dtype;         /* rows and cache: SCHED_PD_F32, SCHED_PD_BF16 or SCHED_PD_F16 */
+  uint32_t w_dtype;       /* weights, the same choice */
+  uint32_t num_tokens;
+  uint32_t num_q_heads, num_kv_heads;
+  uint32_t head_dim;      /* multiple of 4, <= 256 */
+  uint32_t rot_dim;       /* even, 2 .. head_dim */
+  uint32_t interleaved;
+  uint32_t pos_i64;       /* positions are int64 (else int32) */
+  uint32_t max_pos;       /* rows of cos_sin */
+  float eps;
+  const void *q, *k, *v;  /* row i, head h: base + i*tok_stride + h*head_stride, dims contiguous */
+  int64_t q_tok_stride, q_head_stride, k_tok_stride, k_head_stride, v_tok_stride, v_head_stride;
+  void *q_out, *k_out;
+  int64_t qo_tok_stride, qo_head_stride, ko_tok_stride, ko_head_stride;
+  const void *q_weight, *k_weight; /* [head_dim] or NULL */
+  const void *positions;  /* [num_tokens] */
+  const float *cos_sin;   /* [max_pos][rot_dim], rows cs_stride floats apart */
+  int64_t cs_stride;
+  uint32_t *errors;
+  /* the cache; k_pool NULL = none */
+  uint32_t num_requests, page_size, bt_stride;
+  uint32_t max_append;    /* >= every n_r (sizes the grid; 0 = num_tokens) */
+  uint64_t num_pages;
+  const int32_t *append_indptr, *ctx_lens, *block_table, *page_indptr;
+  void *k_pool, *v_pool;
+  int64_t kp_page_stride, kp_head_stride, kp_tok_stride; /* elements, dims contiguous */
+  int64_t vp_page_stride, vp_head_stride, vp_tok_stride;
+} SchedRotaryArgs;
+
+/* Fill *a with defaults (ABI version, BF16 rows, F32 weights, eps 1e-6). */
+void sched_rotary_default_args(SchedRotaryArgs *a);
+
+/* Run it on `stream`, one launch. Returns 0, or -1 with sched_pd_last_error() set. */
+int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream);
+
+/* ---- eviction by accumulated attention weight -------------------------------- */
+
+#define SCHED_EVICT_ABI_VERSION 1u
+
+/* Cut requests to their keep_lens, per kv-head, in place. With n = ctx_lens[r] and m =
+ * min(n, keep_lens[r], max_keep), head h keeps the first `sink` tokens, the last
+ * `recent` (the recent ones first where m holds fewer than both) and, of those
+ * between, the m - sink - recent with the largest weights; of equal weights the token
+ * in the lower slot, NaN below every number. The kept tokens keep their order and move
+ * to slots 0 .. m-1 of the request's pages, keys, values and weights alike (weights
+ * to weights_out, which may be weights). kept[r][h][0..m-1] are the slots they had, the rest of
+ * that row -1. Slots from m on, and requests with m == n, keep what they held; the
+ * caller's lengths become m. Keys carry their rotation along: positions do not
+ * follow the slots.
+ *
+ * fp8: a page's scale becomes the largest of the scales its tokens had, and codes from
+ * pages of another scale s are encoded anew, e4m3(clamp(c * s / scale)): exact for
+ * power-of-two scales unless a code drops into the subnormal range. NaN codes
+ * stay NaN.
+ *
+ * A request that has a page id outside [0, num_pages), or fewer table entries than
+ * its context needs, is left alone: its kept rows are -1, and `errors` (NULL =
+ * none) counts one for each of its kv-heads. Pages of one call belong to one
+ * request each. No counterpart in the reference. */
+typedef struct SchedEvictArgs {
+  uint32_t abi_version;   /* SCHED_EVICT_ABI_VERSION */
+  uint32_t kv_dtype;
+  uint32_t num_requests, num_kv_heads;
+  uint32_t head_dim;      /* multiple of 4, <= 256 */
+  uint32_t page_size;     /* multiple of 4, <= 256 */
+  uint32_t bt_stride;
+  uint32_t max_pages;     /* table width (2-D), or the page list's length */
+  uint32_t max_keep;
+  uint32_t sink, recent;
+  uint32_t _pad0;
+  uint64_t num_pages;
+  void *k_pool, *v_pool;
+  int64_t k_page_stride, k_head_stride, k_tok_stride;
+  int64_t v_page_stride, v_head_stride, v_tok_stride, v_dim_stride;
+  float *k_scale, *v_scale;
+  const float *weights;   /* weights[page*w_page_stride + h*w_head_stride + slot] */
+  float *weights_out;     /* the same strides */
+  int64_t w_page_stride, w_head_stride;
+  const int32_t *block_table, *page_indptr;
+  const int32_t *ctx_lens, *keep_lens;
+  int32_t *kept;          /* [num_requests][num_kv_heads][max_keep], written */
+  uint32_t *errors;
+  void *workspace;        /* sched_kv_evict_workspace_bytes, 256-byte aligned, any contents */
+  uint64_t workspace_bytes;
+} SchedEvictArgs;
+
+/* Fill *a with defaults (ABI version, BF16, the rest 0/NULL). */
+void sched_evict_default_args(SchedEvictArgs *a);
+
+/* Run it on `stream`. Returns 0, or -1 with sched_pd_last_error() set. */
+int sched_kv_evict(const SchedEvictArgs *a, void *stream);
+
+/* Bytes of workspace that call needs (0: none), -1 on invalid arguments (the pointers
+ * are not looked at). */
+int64_t sched_kv_evict_workspace_bytes(const SchedEvictArgs *a);
+
 #ifdef __cplusplus
 }
 #endif

@@ -416,6 +416,90 @@ int sched_pd_read_probe_blocks(const void *buf, uint64_t bytes, const int32_t *b
 /* Last error text of this thread ("" if none). */
 const char *sched_pd_last_error(void);
 
+/* ---- 2b. decode with attention maps handed on ------------------------------ */
+
+#define SCHED_MAPS_ABI_VERSION 1u
+
+/* op */
+#define SCHED_MAPS_WEIGHTED 0u /* the decode, and each token's attention weight added up */
+#define SCHED_MAPS_DIFF 1u     /* the difference of two softmax maps times V */
+
+/* One decode step whose attention maps are used beyond softmax(q K^T) V. Pools,
+ * strides, page tables and context lengths are SchedDecodeArgs'; no levers.
+ *
+ * SCHED_MAPS_WEIGHTED: out as SCHED_PD_SOFTMAX, and for every token t of request r
+ * and every kv-head h
+ *   W[r,h,t] = (t < counted[r] ? decay * W[r,h,t] : 0) + sum over h's q-heads of softmax(t)
+ * where W[r,h,t] is weights[page*w_page_stride + h*w_head_stride + slot] of the
+ * token's page and slot. counted NULL: every token has a weight already. What
+ * lies in slots from counted[r] on is not read (a page taken from the free list
+ * needs no clearing), and slots past the context are left as they are. Pages of
+ * one call belong to one request each.
+ *
+ * SCHED_MAPS_DIFF: q = [q1 | q2] and k = [k1 | k2] hold two maps of head_dim / 2 dims
+ * side by side, V rows head_dim dims:
+ *   o = (softmax(s q1.K1) - lam[hq] softmax(s q2.K2)) V,  s = sm_scale or (head_dim/2)^-1/2
+ *   out = out_scale * o                                        (norm_weight NULL)
+ *       = out_scale * norm_weight * o / sqrt(mean(o^2) + eps)  otherwise
+ *
+ * A request without tokens gives NaN rows (0/0), as the decode's. Scores, maps,
+ * sums and weights are held in 32 bits. No counterpart in the reference. */
+typedef struct SchedMapsArgs {
+  uint32_t abi_version;  /* SCHED_MAPS_ABI_VERSION */
+  uint32_t op;
+  uint32_t kv_dtype;     /* F32, BF16, F16 or FP8_E4M3 */
+  uint32_t q_dtype;      /* F32, BF16 or F16 */
+  uint32_t o_dtype;      /* F32, BF16 or F16 */
+  uint32_t num_requests;
+  uint32_t num_q_heads;  /* multiple of num_kv_heads; at most 16 (DIFF: 8) per kv-head */
+  uint32_t num_kv_heads;
+  uint32_t head_dim;     /* WEIGHTED: 32, 64, 128 or 256; DIFF: 64, 128 or 256 */
+  uint32_t page_size;    /* multiple of 16, at most 256 */
+  uint32_t bt_stride;
+  uint32_t max_pages;    /* table width, or the page list's length with page_indptr: a
+                            request's pages past it are not read */
+  uint32_t flags;        /* SCHED_PD_FLAG_FORCE_VALU or 0 */
+  float sm_scale;        /* 0 = the default above */
+  float decay;           /* WEIGHTED */
+  float eps, out_scale;  /* DIFF */
+  uint64_t num_pages;    /* pool pages; a page id outside [0, num_pages) is not followed */
+  const void *q;         /* [num_requests][num_q_heads][head_dim] */
+  void *out;             /* the same shape */
+  const void *k_pool;
+  const void *v_pool;
+  int64_t k_page_stride, k_head_stride, k_tok_stride;
+  int64_t v_page_stride, v_head_stride, v_tok_stride, v_dim_stride;
+  const float *k_scale;  /* fp8: [num_pages*num_kv_heads], as SchedDecodeArgs */
+  const float *v_scale;
+  const int32_t *block_table;
+  const int32_t *page_indptr; /* NULL = 2-D block table */
+  const int32_t *ctx_lens;
+  float *weights;             /* WEIGHTED */
+  int64_t w_page_stride, w_head_stride;
+  const int32_t *counted;     /* WEIGHTED: [num_requests] or NULL */
+  const float *lam;           /* DIFF: [num_q_heads] */
+  const float *norm_weight;   /* DIFF: [head_dim] or NULL */
+  void *workspace;            /* sched_decode_maps_workspace_bytes, 256-byte aligned; what it */
+  uint64_t workspace_bytes;   /* holds before and after a call means nothing */
+} SchedMapsArgs;
+
+/* Fill *a with defaults (ABI version, BF16, decay 1, eps 1e-5, out_scale 1, the
+ * rest 0/NULL). */
+void sched_maps_default_args(SchedMapsArgs *a);
+
+/* Run one such step on `stream`. Asynchronous, nothing allocated: it may be
+ * captured in a graph. Calls that share a workspace must not overlap. Returns 0 or
+ * a hipError_t code. */
+int sched_decode_maps(const SchedMapsArgs *a, void *stream);
+
+/* Bytes of workspace that call needs, -1 on invalid arguments (workspace,
+ * workspace_bytes and the pointers are not looked at). */
+int64_t sched_decode_maps_workspace_bytes(const SchedMapsArgs *a);
+
+/* Which kernel streams the cache: 0 = the general VALU kernel, 1 = MFMA, -1 =
+ * invalid arguments. */
+int sched_decode_maps_kernel_kind(const SchedMapsArgs *a);
+
 /* ---- 3. reference JIT-kernel launcher ------------------------------------ */
 
 /* reference python/kernels/paged_softmax.cu:47-54: fp32 online-softmax decode,

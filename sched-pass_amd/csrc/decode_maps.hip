@@ -1,0 +1,447 @@
+// decode_maps.hip -- decode steps whose attention maps are used beyond softmax(q
+// K^T) V (sched_decode_maps): each token's weight added up, or the difference of
+// two maps. Two launches: a kernel that streams the cache once (chunks of tasks
+// over the card), and one that joins the chunks and writes what the operator
+// hands on (maps.h has the mathematics).
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+
+#include "maps.h"
+#include "rt_internal.h"
+
+using namespace schedpd;
+
+namespace {
+
+constexpr int kBlock = 256;
+constexpr uint32_t kMostRows = 16;
+
+template <typename T> __device__ __forceinline__ float val(const T *p);
+template <> __device__ __forceinline__ float val(const float *p) { return *p; }
+template <> __device__ __forceinline__ float val(const uint16_t *p) {
+  return bf16_bits_to_f32(*p);
+}
+template <> __device__ __forceinline__ float val(const _Float16 *p) { return (float)*p; }
+template <> __device__ __forceinline__ float val(const uint8_t *p) { return fp8e4m3_to_f32(*p); }
+
+// The general stream: any cache type, layout and strides. A workgroup reads one chunk
+// of one task in tiles of 32 tokens: keys and values go to LDS as fp32; each of the
+// eight 32-lane groups scores the tile's tokens for two rows, in the lanes; then each
+// lane adds the tile's values into one dim of some rows.
+template <typename T, int D, bool DIFF>
+__global__ void __launch_bounds__(kBlock) maps_valu(MapParams P) {
+  constexpr uint32_t TT = 32;                   // tokens of a tile
+  constexpr uint32_t RG = kBlock / (D < kBlock ? D : kBlock); // row groups of the products
+  constexpr uint32_t RPL = kMostRows / RG;      // rows of a lane
+  __shared__ float s_q[kMostRows][D];
+  __shared__ float s_k[TT][D + 1];
+  __shared__ float s_v[TT][D];
+  __shared__ float s_p[kMostRows][TT + 1];
+  __shared__ float s_c[kMostRows];
+  __shared__ int32_t s_page[TT / 4];
+  const uint32_t tid = threadIdx.x, lane32 = tid & 31u, grp = tid >> 5;
+  const uint32_t item = blockIdx.x, task = item / P.nsplit, chunk = item % P.nsplit;
+  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
+  const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
+  const uint64_t first = (uint64_t)chunk * len;
+  if (first >= n && chunk > 0u)
+    return;
+  const uint32_t t0 = (uint32_t)first, t1 = (uint32_t)(first + len < n ? first + len : n);
+  const int64_t row = map_row(P, r);
+  const uint64_t b0 = DIFF ? 0 : blocks_before(P, r);
+
+  // map row 2g + a of the difference holds q-head g's half a, the other half zero
+  for (uint32_t i = tid; i < P.rows * D; i += kBlock) {
+    const uint32_t g = i / D, j = i % D;
+    const uint32_t hq = h * P.G + (DIFF ? g >> 1 : g);
+    const bool in = !DIFF || (j >= D / 2) == (g & 1u);
+    s_q[g][j] = in ? map_load_q(P, ((int64_t)r * P.Hq + hq) * D + j) * P.scale_log2 : 0.f;
+  }
+  float m[2] = {kMInit, kMInit}, l[2] = {0.f, 0.f};
+  float acc[RPL];
+#pragma unroll
+  for (uint32_t i = 0; i < RPL; ++i)
+    acc[i] = 0.f;
+  const uint32_t j0 = tid % (D < kBlock ? D : kBlock), rg = tid / D;
+
+  const T *kp = static_cast<const T *>(P.k_pool) + (int64_t)h * P.khs;
+  const T *vp = static_cast<const T *>(P.v_pool) + (int64_t)h * P.vhs;
+  for (uint32_t tb = t0; tb < t1; tb += TT) {
+    const uint32_t cnt = t1 - tb < TT ? t1 - tb : TT;
+    __syncthreads();
+    // page ids of the tile: at most TT / 16 + 1 pages, pages hold 16 tokens or more
+    const uint32_t pg0 = tb / P.ps, pg1 = (tb + cnt - 1u) / P.ps;
+    if (tid <= pg1 - pg0)
+      s_page[tid] = P.bt[row + pg0 + tid];
+    __syncthreads();
+    for (uint32_t i = tid; i < TT * D; i += kBlock) {
+      const uint32_t t = i / D, j = i % D;
+      float x = 0.f;
+      if (t < cnt) {
+        const uint32_t page = (uint32_t)s_page[(tb + t) / P.ps - pg0], slot = (tb + t) % P.ps;
+        if (page < P.num_pages) {
+          x = val(kp + (int64_t)page * P.kps + (int64_t)slot * P.kts + j);
+          if (sizeof(T) == 1 && P.k_scale)
+            x *= P.k_scale[((int64_t)page * P.Hkv + h) * P.scale_stride];
+        }
+      }
+      s_k[t][j] = x;
+    }
+    // the order of the values' loads follows their layout
+    for (uint32_t i = tid; i < TT * D; i += kBlock) {
+      const uint32_t t = P.vds == 1 ? i / D : i % TT, j = P.vds == 1 ? i % D : i / TT;
+      float x = 0.f;
+      if (t < cnt) {
+        const uint32_t page = (uint32_t)s_page[(tb + t) / P.ps - pg0], slot = (tb + t) % P.ps;
+        if (page < P.num_pages) {
+          x = val(vp + (int64_t)page * P.vps + (int64_t)slot * P.vts + (int64_t)j * P.vds);
+          if (sizeof(T) == 1 && P.v_scale)
+            x *= P.v_scale[((int64_t)page * P.Hkv + h) * P.scale_stride];
+        }
+      }
+      s_v[t][j] = x;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < 2; ++k) {
+      const uint32_t g = grp + 8u * k;
+      if (g >= P.rows)
+        continue;
+      float a = 0.f;
+      const uint32_t j_lo = DIFF && (g & 1u) ? D / 2 : 0u, j_hi = DIFF && !(g & 1u) ? D / 2 : D;
+      for (uint32_t j = j_lo; j < j_hi; ++j)
+        a += s_q[g][j] * s_k[lane32][j];
+      const bool in = lane32 < cnt;
+      const float s = in ? a : kNegInf;
+      if (!DIFF && in) {
+        const uint32_t t = tb + lane32;
+        if (b0 + t / 16u < P.score_blocks)
+          score_block(P, b0, t / 16u, h)[g * 16u + (t & 15u)] = s;
+      }
+      float mx = s;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        mx = fmaxf(mx, __shfl_xor(mx, o, 32));
+      const float mn = fmaxf(m[k], mx), c = __builtin_amdgcn_exp2f(m[k] - mn);
+      const float p = in ? __builtin_amdgcn_exp2f(s - mn) : 0.f;
+      float sum = p;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1)
+        sum += __shfl_xor(sum, o, 32);
+      m[k] = mn;
+      l[k] = l[k] * c + sum;
+      s_p[g][lane32] = p;
+      if (lane32 == 0)
+        s_c[g] = c;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t i = 0; i < RPL; ++i) {
+      const uint32_t g = rg + RG * i;
+      if (g >= P.rows)
+        continue;
+      float a = acc[i] * s_c[g];
+      for (uint32_t t = 0; t < cnt; ++t)
+        a += s_p[g][t] * s_v[t][j0];
+      acc[i] = a;
+    }
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 2; ++k) {
+    const uint32_t g = grp + 8u * k;
+    if (g < P.rows && lane32 == 0) {
+      float *ml = P.ml + ((uint64_t)item * P.rows + g) * 2u;
+      ml[0] = m[k];
+      ml[1] = l[k];
+    }
+  }
+#pragma unroll
+  for (uint32_t i = 0; i < RPL; ++i) {
+    const uint32_t g = rg + RG * i;
+    if (g < P.rows)
+      P.acc[((uint64_t)item * P.rows + g) * D + j0] = acc[i];
+  }
+}
+
+// The join: workgroup (task, b). b = 0 writes the task's outputs; the weights' token
+// blocks are dealt out over all b.
+template <bool DIFF> __global__ void __launch_bounds__(kBlock) maps_join(MapParams P) {
+  __shared__ float s_m[kMostRows], s_li[kMostRows], s_sum[kBlock / 64];
+  const uint32_t tid = threadIdx.x, task = blockIdx.x;
+  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
+  const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
+  const uint32_t nch = n == 0u ? 1u : (n + len - 1u) / len;
+  const uint64_t item0 = (uint64_t)task * P.nsplit;
+  if (tid < P.rows) {
+    const float *ml = P.ml + (item0 * P.rows + tid) * 2u;
+    float M = ml[0];
+    for (uint32_t c = 1; c < nch; ++c)
+      M = fmaxf(M, ml[(uint64_t)c * P.rows * 2u]);
+    float L = 0.f;
+    for (uint32_t c = 0; c < nch; ++c) {
+      const float *e = ml + (uint64_t)c * P.rows * 2u;
+      L += e[1] * __builtin_amdgcn_exp2f(e[0] - M);
+    }
+    s_m[tid] = M;
+    s_li[tid] = 1.f / L;
+  }
+  __syncthreads();
+  if (blockIdx.y == 0) {
+    const uint32_t D = P.D;
+    auto joined = [&](uint32_t g, uint32_t j) {
+      float o = 0.f;
+      for (uint32_t c = 0; c < nch; ++c) {
+        const uint64_t e = (item0 + c) * P.rows + g;
+        o += P.acc[e * D + j] * __builtin_amdgcn_exp2f(P.ml[e * 2u] - s_m[g]);
+      }
+      return o * s_li[g];
+    };
+    if constexpr (!DIFF) {
+      for (uint32_t i = tid; i < P.G * D; i += kBlock)
+        map_store(P, ((int64_t)r * P.Hq + h * P.G + i / D) * D + i % D, n ? joined(i / D, i % D)
+                                                                         : __builtin_nanf(""));
+    } else {
+      for (uint32_t g = 0; g < P.G; ++g) {
+        const uint32_t hq = h * P.G + g;
+        float o = 0.f;
+        if (tid < D)
+          o = joined(2u * g, tid) - P.lam[hq] * joined(2u * g + 1u, tid);
+        float inv = 1.f;
+        if (P.nw) {
+          float ss = o * o;
+#pragma unroll
+          for (int k = 32; k > 0; k >>= 1)
+            ss += __shfl_xor(ss, k);
+          __syncthreads(); // the previous head's sums have been read
+          if ((tid & 63u) == 0u)
+            s_sum[tid >> 6] = ss;
+          __syncthreads();
+          ss = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+          inv = rsqrtf(ss / (float)D + P.eps);
+        }
+        if (tid < D)
+          map_store(P, ((int64_t)r * P.Hq + hq) * D + tid,
+                    n ? o * inv * (P.nw ? P.nw[tid] : 1.f) * P.mul : __builtin_nanf(""));
+      }
+    }
+  }
+  if constexpr (!DIFF) {
+    const uint64_t b0 = blocks_before(P, r);
+    const int64_t row = map_row(P, r);
+    const int64_t cnt = P.counted ? (int64_t)P.counted[r] : (int64_t)n;
+    for (uint32_t t = blockIdx.y * kBlock + tid; t < n; t += gridDim.y * kBlock) {
+      const uint32_t page = (uint32_t)P.bt[row + t / P.ps];
+      if (page >= P.num_pages || b0 + t / 16u >= P.score_blocks)
+        continue;
+      const float *s = score_block(P, b0, t / 16u, h) + (t & 15u);
+      float *w = P.w + (int64_t)page * P.w_ps + (int64_t)h * P.w_hs + t % P.ps;
+      float a = 0.f;
+      for (uint32_t g = 0; g < P.rows; ++g)
+        a += __builtin_amdgcn_exp2f(s[g * 16u] - s_m[g]) * s_li[g];
+      *w = (int64_t)t < cnt ? *w * P.decay + a : a;
+    }
+  }
+}
+
+uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
+
+uint64_t elem_bytes(uint32_t dt) {
+  return dt == SCHED_PD_F32 ? 4u : dt == SCHED_PD_FP8_E4M3 ? 1u : 2u;
+}
+
+// What a call's shape decides: how far tasks are split, and the workspace.
+struct Plan {
+  uint32_t rows, nsplit, least;
+  uint64_t score_blocks, ml_off, acc_off, total;
+};
+
+int check_shape(const SchedMapsArgs *a) {
+  if (!a)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: args is NULL");
+  if (a->abi_version != SCHED_MAPS_ABI_VERSION)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: abi_version %u, library has %u",
+                     a->abi_version, SCHED_MAPS_ABI_VERSION);
+  if (a->op > SCHED_MAPS_DIFF)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: op %u", a->op);
+  auto float_dt = [](uint32_t dt) {
+    return dt == SCHED_PD_F32 || dt == SCHED_PD_BF16 || dt == SCHED_PD_F16;
+  };
+  if (a->kv_dtype > SCHED_PD_F16 || !float_dt(a->q_dtype) || !float_dt(a->o_dtype))
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: dtypes (kv %u, q %u, out %u)",
+                     a->kv_dtype, a->q_dtype, a->o_dtype);
+  if (a->num_kv_heads == 0 || a->num_q_heads == 0 || a->num_q_heads % a->num_kv_heads)
+    return set_error(hipErrorInvalidValue,
+                     "sched_decode_maps: num_q_heads %u is not a multiple of num_kv_heads %u",
+                     a->num_q_heads, a->num_kv_heads);
+  const bool diff = a->op == SCHED_MAPS_DIFF;
+  const uint32_t G = a->num_q_heads / a->num_kv_heads;
+  if (G > (diff ? kMostRows / 2 : kMostRows))
+    return set_error(hipErrorInvalidValue,
+                     "sched_decode_maps: %u q-heads per kv-head, at most %u supported", G,
+                     diff ? kMostRows / 2 : kMostRows);
+  const uint32_t d = a->head_dim;
+  if (!(d == 64 || d == 128 || d == 256 || (d == 32 && !diff)))
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: head_dim %u (supported: %s64, 128, "
+                                           "256)", d, diff ? "" : "32, ");
+  if (a->page_size == 0 || a->page_size % 16 || a->page_size > 256)
+    return set_error(hipErrorInvalidValue,
+                     "sched_decode_maps: page_size %u (multiple of 16, at most 256)",
+                     a->page_size);
+  if (a->flags & ~SCHED_PD_FLAG_FORCE_VALU)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: flags 0x%x (FORCE_VALU or 0)",
+                     a->flags);
+  if (a->num_pages == 0 || a->num_pages > 0x7fffffffull)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: num_pages %llu",
+                     (unsigned long long)a->num_pages);
+  if ((uint64_t)a->num_requests * a->num_kv_heads > (1u << 24) ||
+      (uint64_t)a->max_pages * a->page_size > 0x7fffffffull)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: %u requests x %u kv-heads, tables "
+                                           "of %u pages", a->num_requests, a->num_kv_heads,
+                     a->max_pages);
+  return 0;
+}
+
+// Chunks fill the card this many times over; none is shorter than kLeastTokens.
+constexpr uint32_t kItems = 1024, kLeastTokens = 256, kMostSplit = 64;
+
+Plan plan_of(const SchedMapsArgs *a) {
+  Plan p{};
+  const uint64_t tasks = std::max<uint64_t>(1, (uint64_t)a->num_requests * a->num_kv_heads);
+  const uint64_t longest = (uint64_t)a->max_pages * a->page_size;
+  p.rows = a->num_q_heads / a->num_kv_heads * (a->op == SCHED_MAPS_DIFF ? 2u : 1u);
+  p.least = kLeastTokens;
+  const uint64_t want = (kItems + tasks - 1) / tasks, can = (longest + p.least - 1) / p.least;
+  p.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, can, kMostSplit}));
+  if (a->op == SCHED_MAPS_WEIGHTED) {
+    // a call's pages are distinct: never more of them than the pool has
+    uint64_t pages = a->page_indptr ? a->max_pages : (uint64_t)a->num_requests * a->max_pages;
+    pages = std::min<uint64_t>(pages, a->num_pages);
+    p.score_blocks = pages * (a->page_size / 16u);
+  }
+  p.ml_off = up256(p.score_blocks * a->num_kv_heads * p.rows * 64u);
+  p.acc_off = p.ml_off + up256(tasks * p.nsplit * p.rows * 8u);
+  p.total = p.acc_off + tasks * p.nsplit * p.rows * a->head_dim * 4u;
+  return p;
+}
+
+typedef void (*StreamFn)(MapParams);
+
+template <typename T> StreamFn valu_of(uint32_t d, bool diff) {
+  switch (d) {
+  case 32: return maps_valu<T, 32, false>;
+  case 64: return diff ? maps_valu<T, 64, true> : maps_valu<T, 64, false>;
+  case 128: return diff ? maps_valu<T, 128, true> : maps_valu<T, 128, false>;
+  default: return diff ? maps_valu<T, 256, true> : maps_valu<T, 256, false>;
+  }
+}
+
+} // namespace
+
+extern "C" {
+
+void sched_maps_default_args(SchedMapsArgs *a) {
+  if (!a)
+    return;
+  *a = SchedMapsArgs{};
+  a->abi_version = SCHED_MAPS_ABI_VERSION;
+  a->kv_dtype = a->q_dtype = a->o_dtype = SCHED_PD_BF16;
+  a->decay = 1.f;
+  a->eps = 1e-5f;
+  a->out_scale = 1.f;
+}
+
+int64_t sched_decode_maps_workspace_bytes(const SchedMapsArgs *a) {
+  if (check_shape(a))
+    return -1;
+  return (int64_t)plan_of(a).total;
+}
+
+int sched_decode_maps_kernel_kind(const SchedMapsArgs *a) {
+  if (check_shape(a))
+    return -1;
+  return 0;
+}
+
+int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
+  if (int rc = check_shape(a))
+    return rc;
+  if (a->num_requests == 0)
+    return 0;
+  const bool diff = a->op == SCHED_MAPS_DIFF;
+  if (!a->q || !a->out || !a->k_pool || !a->v_pool || !a->block_table || !a->ctx_lens)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: a required pointer is NULL");
+  if (diff ? a->lam == nullptr : a->weights == nullptr)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: %s is required",
+                     diff ? "lam" : "weights");
+  if (a->kv_dtype == SCHED_PD_FP8_E4M3 && (!a->k_scale || !a->v_scale))
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: an fp8 cache needs k_scale and "
+                                           "v_scale");
+  if (!a->page_indptr && a->bt_stride < a->max_pages)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: bt_stride %u below max_pages %u",
+                     a->bt_stride, a->max_pages);
+  if (a->v_tok_stride != 1 && a->v_dim_stride != 1)
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: V needs v_tok_stride == 1 "
+                                           "(d-major) or v_dim_stride == 1 (token-major)");
+  const uintptr_t eb = elem_bytes(a->kv_dtype);
+  if ((uintptr_t)a->k_pool % eb || (uintptr_t)a->v_pool % eb ||
+      (uintptr_t)a->q % elem_bytes(a->q_dtype) || (uintptr_t)a->out % elem_bytes(a->o_dtype))
+    return set_error(hipErrorInvalidValue,
+                     "sched_decode_maps: a tensor is not aligned to its elements");
+  const Plan plan = plan_of(a);
+  if (!a->workspace || a->workspace_bytes < plan.total || ((uintptr_t)a->workspace & 255u))
+    return set_error(hipErrorInvalidValue, "sched_decode_maps: needs a 256-byte aligned workspace "
+                                           "of %llu bytes (got %llu)",
+                     (unsigned long long)plan.total, (unsigned long long)a->workspace_bytes);
+  MapParams P{};
+  P.q = a->q, P.out = a->out, P.k_pool = a->k_pool, P.v_pool = a->v_pool;
+  P.kps = a->k_page_stride, P.khs = a->k_head_stride, P.kts = a->k_tok_stride;
+  P.vps = a->v_page_stride, P.vhs = a->v_head_stride, P.vts = a->v_tok_stride;
+  P.vds = a->v_dim_stride;
+  P.k_scale = a->k_scale, P.v_scale = a->v_scale;
+  P.scale_stride = (a->k_scale != nullptr && a->v_scale == a->k_scale + 1) ? 2u : 1u;
+  P.bt = a->block_table, P.indptr = a->page_indptr, P.ctx = a->ctx_lens;
+  P.R = a->num_requests, P.Hq = a->num_q_heads, P.Hkv = a->num_kv_heads;
+  P.G = a->num_q_heads / a->num_kv_heads, P.rows = plan.rows;
+  P.D = a->head_dim, P.ps = a->page_size, P.bt_stride = a->bt_stride;
+  P.max_pages = a->max_pages, P.num_pages = (uint32_t)a->num_pages;
+  P.q_dtype = a->q_dtype, P.o_dtype = a->o_dtype;
+  P.nsplit = plan.nsplit, P.least = plan.least;
+  const float dims = (float)(diff ? a->head_dim / 2u : a->head_dim);
+  P.scale_log2 = (a->sm_scale != 0.f ? a->sm_scale : 1.0f / std::sqrt(dims)) *
+                 1.4426950408889634f;
+  P.w = a->weights, P.w_ps = a->w_page_stride, P.w_hs = a->w_head_stride;
+  P.counted = a->counted, P.decay = a->decay;
+  P.lam = a->lam, P.nw = a->norm_weight, P.eps = a->eps, P.mul = a->out_scale;
+  uint8_t *ws = static_cast<uint8_t *>(a->workspace);
+  P.scores = reinterpret_cast<float *>(ws), P.score_blocks = plan.score_blocks;
+  P.ml = reinterpret_cast<float *>(ws + plan.ml_off);
+  P.acc = reinterpret_cast<float *>(ws + plan.acc_off);
+
+  const uint32_t tasks = P.R * P.Hkv;
+  StreamFn fn = a->kv_dtype == SCHED_PD_F32    ? valu_of<float>(P.D, diff)
+                : a->kv_dtype == SCHED_PD_BF16 ? valu_of<uint16_t>(P.D, diff)
+                : a->kv_dtype == SCHED_PD_F16  ? valu_of<_Float16>(P.D, diff)
+                                               : valu_of<uint8_t>(P.D, diff);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  hipLaunchKernelGGL(fn, dim3(tasks * P.nsplit), dim3(kBlock), 0, s, P);
+  hipError_t e = hipGetLastError();
+  if (e == hipSuccess) {
+    uint32_t by = 1;
+    if (!diff) {
+      const uint64_t longest = (uint64_t)P.max_pages * P.ps;
+      by = (uint32_t)std::max<uint64_t>(
+          1, std::min<uint64_t>((longest + 4 * kBlock - 1) / (4 * kBlock), 4096u / tasks + 1u));
+    }
+    hipLaunchKernelGGL(diff ? maps_join<true> : maps_join<false>, dim3(tasks, by), dim3(kBlock), 0,
+                       s, P);
+    e = hipGetLastError();
+  }
+  if (e != hipSuccess)
+    return set_error(e, "sched_decode_maps: launch failed: %s", hipGetErrorString(e));
+  return 0;
+}
+
+} // extern "C"

@@ -1,0 +1,104 @@
+// maps.h -- what the kernels of the decode with handed-on attention maps share
+// (sched_decode_maps): the parameter block, how a task is cut into chunks, and
+// where scores and partial results lie.
+//
+// A map row is one softmax: q-head g of a kv-head's group (weighted), or map a of
+// q-head g as row 2g + a (difference). Per row the stream of a task's tokens gives
+// the running maximum m and sum l of 2^s (s = score * log2(e) / scale) and the
+// unnormalised products O = sum 2^(s - m) v. Chunks of a task join as
+//   M = max m_c,  L = sum l_c 2^(m_c - M),  O = sum O_c 2^(m_c - M).
+// The weights need every token's 2^(s - M) / L, which is known only when all of
+// the task has been read: the stream leaves its scores behind in 32 bits, and the
+// join turns them into weights.
+#pragma once
+
+#include "common.h"
+
+namespace schedpd {
+
+struct MapParams {
+  const void *q;
+  void *out;
+  const void *k_pool, *v_pool;
+  int64_t kps, khs, kts;
+  int64_t vps, vhs, vts, vds;
+  const float *k_scale, *v_scale;
+  uint32_t scale_stride;
+  const int32_t *bt, *indptr, *ctx;
+  uint32_t R, Hq, Hkv, G, rows; // rows: maps per kv-head (G, or 2 G)
+  uint32_t D, ps, bt_stride, max_pages, num_pages;
+  uint32_t q_dtype, o_dtype;
+  uint32_t nsplit, least; // most chunks of a task; least tokens of one (a multiple of 64)
+  float scale_log2;
+  // weighted
+  float *w;
+  int64_t w_ps, w_hs;
+  const int32_t *counted;
+  float decay;
+  float *scores;       // [16-token block of the batch][kv-head][row][16]
+  uint64_t score_blocks; // blocks it holds
+  // difference
+  const float *lam, *nw;
+  float eps, mul;
+  // partials of chunk c of task t, item t * nsplit + c: (m, l) per row, O per row
+  float *ml, *acc;
+};
+
+// A request's tokens: its context, as far as its table reaches.
+__device__ __forceinline__ uint32_t map_tokens(const MapParams &P, uint32_t r) {
+  const int32_t c = P.ctx[r];
+  uint32_t pages = P.max_pages;
+  if (P.indptr) {
+    const int32_t have = P.indptr[r + 1] - P.indptr[r];
+    pages = have > 0 ? (uint32_t)have : 0u;
+  }
+  const uint64_t cap = (uint64_t)pages * P.ps;
+  return c <= 0 ? 0u : (uint64_t)c < cap ? (uint32_t)c : (uint32_t)cap;
+}
+
+__device__ __forceinline__ int64_t map_row(const MapParams &P, uint32_t r) {
+  return P.indptr ? (int64_t)P.indptr[r] : (int64_t)r * P.bt_stride;
+}
+
+// Tokens of a chunk of an n-token task: nsplit equal ones, none below `least`,
+// in multiples of 64.
+__device__ __forceinline__ uint32_t map_chunk(const MapParams &P, uint32_t n) {
+  const uint32_t even = (uint32_t)(((uint64_t)n + P.nsplit - 1u) / P.nsplit);
+  const uint32_t c = even > P.least ? even : P.least;
+  return (c + 63u) & ~63u;
+}
+
+// Score blocks of the requests before r (one wave or more; every lane takes part
+// and gets the sum).
+__device__ __forceinline__ uint64_t blocks_before(const MapParams &P, uint32_t r) {
+  unsigned long long s = 0;
+  for (uint32_t i = threadIdx.x & 63u; i < r; i += 64u)
+    s += (map_tokens(P, i) + 15u) / 16u;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    s += __shfl_xor(s, o);
+  return s;
+}
+
+// Score of row g, token i of a block: block blk of the request whose first block is b0.
+__device__ __forceinline__ float *score_block(const MapParams &P, uint64_t b0, uint32_t blk,
+                                              uint32_t h) {
+  return P.scores + ((b0 + blk) * P.Hkv + h) * P.rows * 16u;
+}
+
+__device__ __forceinline__ void map_store(const MapParams &P, int64_t i, float v) {
+  if (P.o_dtype == SCHED_PD_F32)
+    static_cast<float *>(P.out)[i] = v;
+  else if (P.o_dtype == SCHED_PD_F16)
+    static_cast<_Float16 *>(P.out)[i] = (_Float16)v;
+  else
+    static_cast<uint16_t *>(P.out)[i] = f32_to_bf16_rne(v);
+}
+
+__device__ __forceinline__ float map_load_q(const MapParams &P, int64_t i) {
+  return P.q_dtype == SCHED_PD_F32   ? static_cast<const float *>(P.q)[i]
+         : P.q_dtype == SCHED_PD_F16 ? (float)static_cast<const _Float16 *>(P.q)[i]
+                                     : bf16_bits_to_f32(static_cast<const uint16_t *>(P.q)[i]);
+}
+
+} // namespace schedpd

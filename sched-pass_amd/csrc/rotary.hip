@@ -1,0 +1,305 @@
+// rotary.hip -- norm of queries and keys per head with the position rotation in the
+// same pass (sched_qk_norm_rope), the key and value rows straight into the paged
+// cache if there is one.
+//
+// Per row x of d dims (one token, one head), in fp32:
+//   x' = x * w * rsqrt(mean(x^2) + eps),
+//   (y_a, y_b) = (x'_a c - x'_b s, x'_b c + x'_a s) for the rotated pairs,
+// rounded once. Bound by its bytes: each row is read once and written once, the
+// token's angles are read once per workgroup and shared by its heads through the
+// cache.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "common.h"
+#include "rt_internal.h"
+#include "sched_kv.h"
+
+using namespace schedpd;
+
+namespace {
+
+constexpr int kBlock = 256;
+
+struct RParams {
+  const void *q, *k, *v;
+  int64_t q_ts, q_hs, k_ts, k_hs, v_ts, v_hs;
+  void *qo, *ko;
+  int64_t qo_ts, qo_hs, ko_ts, ko_hs;
+  const void *qw, *kw;
+  const void *pos;
+  const float *cs;
+  int64_t cs_stride;
+  uint32_t *errors;
+  uint32_t T, Hq, Hkv, d, rot, max_pos;
+  uint32_t w_dtype, inter, pos64;
+  float eps;
+  // the cache (kp == nullptr: none)
+  void *kp, *vp;
+  int64_t kps, khs, kts, vps, vhs, vts;
+  const int32_t *app, *ctx, *table, *pind;
+  uint32_t ps, bt_stride;
+  uint64_t num_pages;
+};
+
+template <int DT> __device__ __forceinline__ float ld(const void *p, int64_t i) {
+  if constexpr (DT == SCHED_PD_F32)
+    return static_cast<const float *>(p)[i];
+  else if constexpr (DT == SCHED_PD_BF16)
+    return bf16_bits_to_f32(static_cast<const uint16_t *>(p)[i]);
+  else
+    return (float)static_cast<const _Float16 *>(p)[i];
+}
+
+template <int DT> __device__ __forceinline__ void st(void *p, int64_t i, float v) {
+  if constexpr (DT == SCHED_PD_F32)
+    static_cast<float *>(p)[i] = v;
+  else if constexpr (DT == SCHED_PD_BF16)
+    static_cast<uint16_t *>(p)[i] = f32_to_bf16_rne(v);
+  else
+    static_cast<_Float16 *>(p)[i] = (_Float16)v;
+}
+
+__device__ __forceinline__ float load_w(const RParams &P, const void *w, uint32_t j) {
+  return P.w_dtype == SCHED_PD_F32    ? ld<SCHED_PD_F32>(w, j)
+         : P.w_dtype == SCHED_PD_BF16 ? ld<SCHED_PD_BF16>(w, j)
+                                      : ld<SCHED_PD_F16>(w, j);
+}
+
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1)
+    x += __shfl_xor(x, o);
+  return x;
+}
+
+// Where a token's cache rows go: the page, and the slot in it; page -1 = nowhere.
+struct Place {
+  int64_t page;
+  uint32_t slot;
+};
+
+// The tokens [a0, a0 + n) of one request (the whole batch without a cache).
+struct Span {
+  int64_t a0, n, ctx, row, cap;
+};
+
+__device__ __forceinline__ Span span_of(const RParams &P, uint32_t r) {
+  Span s{0, P.T, 0, 0, 0};
+  if (P.kp == nullptr)
+    return s;
+  const int64_t a0 = P.app[r], a1 = P.app[r + 1];
+  s.a0 = a0 < 0 ? 0 : a0;
+  s.n = (a1 < (int64_t)P.T ? a1 : (int64_t)P.T) - s.a0; // rows outside the sources: skipped
+  s.ctx = P.ctx[r];
+  s.row = P.pind ? (int64_t)P.pind[r] : (int64_t)r * P.bt_stride;
+  s.cap = P.pind ? (int64_t)P.pind[r + 1] - P.pind[r] : (int64_t)P.bt_stride;
+  return s;
+}
+
+__device__ __forceinline__ Place place_of(const RParams &P, const Span &s, int64_t i) {
+  const int64_t at = s.ctx - s.n + i;
+  if (at < 0)
+    return {-1, 0};
+  const int64_t b = at / P.ps;
+  if (b >= s.cap)
+    return {-1, 0};
+  const int32_t page = P.table[s.row + b];
+  if (page < 0 || (uint64_t)page >= P.num_pages)
+    return {-1, 0};
+  return {page, (uint32_t)(at % P.ps)};
+}
+
+__device__ __forceinline__ int64_t position_of(const RParams &P, int64_t tok) {
+  return P.pos64 ? static_cast<const int64_t *>(P.pos)[tok]
+                 : (int64_t) static_cast<const int32_t *>(P.pos)[tok];
+}
+
+// Every shape: one wave per row, element e = lane + 64 i of it in each lane. The
+// rotated partner of an element is read from the row itself.
+template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams P) {
+  const uint32_t lane = threadIdx.x & 63u;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const Span S = span_of(P, blockIdx.x);
+  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), half = P.rot / 2u;
+  for (int64_t i = blockIdx.y; i < S.n; i += gridDim.y) {
+    const int64_t tok = S.a0 + i;
+    const int64_t pos = position_of(P, tok);
+    if (pos < 0 || pos >= (int64_t)P.max_pos) {
+      if (threadIdx.x == 0 && P.errors)
+        atomicAdd(P.errors, 1u);
+      continue;
+    }
+    const float *cs = P.cs + pos * P.cs_stride;
+    Place at{-1, 0};
+    if (P.kp) {
+      at = place_of(P, S, i);
+      if (at.page < 0 && threadIdx.x == 0 && P.errors)
+        atomicAdd(P.errors, P.Hkv);
+    }
+    for (uint32_t row = wave; row < rows; row += kBlock / 64) {
+      const bool isq = row < P.Hq, isv = row >= P.Hq + P.Hkv;
+      const uint32_t h = isq ? row : isv ? row - P.Hq - P.Hkv : row - P.Hq;
+      const void *src = isq ? P.q : isv ? P.v : P.k;
+      const int64_t s0 = isq   ? tok * P.q_ts + h * P.q_hs
+                         : isv ? tok * P.v_ts + h * P.v_hs
+                               : tok * P.k_ts + h * P.k_hs;
+      void *dst;
+      int64_t d0;
+      if (isq) {
+        dst = P.qo, d0 = tok * P.qo_ts + h * P.qo_hs;
+      } else if (P.kp == nullptr) {
+        dst = P.ko, d0 = tok * P.ko_ts + h * P.ko_hs;
+      } else if (at.page < 0) {
+        continue;
+      } else if (isv) {
+        dst = P.vp, d0 = at.page * P.vps + h * P.vhs + at.slot * P.vts;
+      } else {
+        dst = P.kp, d0 = at.page * P.kps + h * P.khs + at.slot * P.kts;
+      }
+      const void *w = isv ? nullptr : isq ? P.qw : P.kw;
+      float x[4], y[4];
+      float ss = 0.f;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t e = lane + 64u * u;
+        x[u] = e < P.d ? ld<DT>(src, s0 + e) : 0.f;
+        // the partner in the rotated pair
+        const uint32_t p = P.inter ? e ^ 1u : e < half ? e + half : e - half;
+        y[u] = !isv && e < P.rot ? ld<DT>(src, s0 + p) : 0.f;
+        ss += x[u] * x[u];
+      }
+      float inv = 1.f;
+      if (w != nullptr)
+        inv = rsqrtf(wave_sum(ss) / (float)P.d + P.eps);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t e = lane + 64u * u;
+        if (e >= P.d)
+          continue;
+        float o = x[u];
+        if (w != nullptr)
+          o *= inv * load_w(P, w, e);
+        if (!isv && e < P.rot) {
+          const uint32_t p = P.inter ? e ^ 1u : e < half ? e + half : e - half;
+          const uint32_t j = P.inter ? e >> 1 : e < half ? e : e - half;
+          const bool first = P.inter ? (e & 1u) == 0u : e < half;
+          const float c = cs[j], s = cs[half + j];
+          const float b = w != nullptr ? y[u] * (inv * load_w(P, w, p)) : y[u];
+          o = first ? o * c - b * s : o * c + b * s;
+        }
+        st<DT>(dst, d0 + e, o);
+      }
+    }
+  }
+}
+
+uint32_t esize(uint32_t dt) { return dt == SCHED_PD_F32 ? 4u : 2u; }
+
+bool is_float(uint32_t dt) {
+  return dt == SCHED_PD_F32 || dt == SCHED_PD_BF16 || dt == SCHED_PD_F16;
+}
+
+} // namespace
+
+extern "C" {
+
+void sched_rotary_default_args(SchedRotaryArgs *a) {
+  if (!a)
+    return;
+  *a = SchedRotaryArgs{};
+  a->abi_version = SCHED_ROTARY_ABI_VERSION;
+  a->dtype = SCHED_PD_BF16;
+  a->w_dtype = SCHED_PD_F32;
+  a->eps = 1e-6f;
+}
+
+int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
+  if (!a)
+    return set_error(-1, "sched_qk_norm_rope: args is NULL");
+  if (a->abi_version != SCHED_ROTARY_ABI_VERSION)
+    return set_error(-1, "sched_qk_norm_rope: abi_version %u, library has %u", a->abi_version,
+                     SCHED_ROTARY_ABI_VERSION);
+  if (!is_float(a->dtype) || !is_float(a->w_dtype))
+    return set_error(-1, "sched_qk_norm_rope: dtypes %u, %u (F32, BF16 or F16)", a->dtype,
+                     a->w_dtype);
+  if (a->num_q_heads == 0 || a->num_kv_heads == 0 || a->num_q_heads > 65535u ||
+      a->num_kv_heads > 65535u)
+    return set_error(-1, "sched_qk_norm_rope: %u query and %u key heads", a->num_q_heads,
+                     a->num_kv_heads);
+  if (a->head_dim == 0 || a->head_dim % 4 || a->head_dim > 256)
+    return set_error(-1, "sched_qk_norm_rope: head_dim %u (multiple of 4, <= 256)", a->head_dim);
+  if (a->rot_dim < 2 || a->rot_dim % 2 || a->rot_dim > a->head_dim)
+    return set_error(-1, "sched_qk_norm_rope: rot_dim %u (even, 2 .. head_dim %u)", a->rot_dim,
+                     a->head_dim);
+  if (!(a->eps >= 0.f))
+    return set_error(-1, "sched_qk_norm_rope: eps %g", (double)a->eps);
+  if (a->num_tokens > 0x7fffffffu)
+    return set_error(-1, "sched_qk_norm_rope: num_tokens %u", a->num_tokens);
+  const bool cache = a->k_pool != nullptr;
+  if (a->num_tokens == 0 || (cache && a->num_requests == 0))
+    return 0;
+  if (!a->q || !a->k || !a->q_out || !a->positions || !a->cos_sin || a->max_pos == 0)
+    return set_error(-1, "sched_qk_norm_rope: a required pointer is NULL (or max_pos 0)");
+  if (!cache && !a->k_out)
+    return set_error(-1, "sched_qk_norm_rope: needs k_out or a cache for the key rows");
+  if (a->cs_stride < (int64_t)a->rot_dim)
+    return set_error(-1, "sched_qk_norm_rope: cs_stride %lld for rot_dim %u",
+                     (long long)a->cs_stride, a->rot_dim);
+  if (cache) {
+    if (!a->v || !a->v_pool || !a->append_indptr || !a->ctx_lens || !a->block_table)
+      return set_error(-1, "sched_qk_norm_rope: a cache needs v, v_pool, append_indptr, "
+                           "ctx_lens and block_table");
+    if (a->page_size == 0 || a->num_pages == 0 || a->num_pages > 0x7fffffffull ||
+        a->num_requests > 0x7fffffffu)
+      return set_error(-1, "sched_qk_norm_rope: page_size %u, num_pages %llu", a->page_size,
+                       (unsigned long long)a->num_pages);
+    if (!a->page_indptr && a->bt_stride == 0)
+      return set_error(-1, "sched_qk_norm_rope: bt_stride is 0 with a 2-D block table");
+  }
+  const uint32_t es = esize(a->dtype);
+  for (const void *p : {a->q, a->k, a->v, (const void *)a->q_out, (const void *)a->k_out,
+                        (const void *)a->k_pool, (const void *)a->v_pool})
+    if ((uintptr_t)p % es)
+      return set_error(-1, "sched_qk_norm_rope: a tensor is not aligned to its elements");
+
+  RParams P{};
+  P.q = a->q, P.k = a->k, P.v = a->v;
+  P.q_ts = a->q_tok_stride, P.q_hs = a->q_head_stride;
+  P.k_ts = a->k_tok_stride, P.k_hs = a->k_head_stride;
+  P.v_ts = a->v_tok_stride, P.v_hs = a->v_head_stride;
+  P.qo = a->q_out, P.ko = a->k_out;
+  P.qo_ts = a->qo_tok_stride, P.qo_hs = a->qo_head_stride;
+  P.ko_ts = a->ko_tok_stride, P.ko_hs = a->ko_head_stride;
+  P.qw = a->q_weight, P.kw = a->k_weight;
+  P.pos = a->positions, P.cs = a->cos_sin, P.cs_stride = a->cs_stride;
+  P.errors = a->errors;
+  P.T = a->num_tokens, P.Hq = a->num_q_heads, P.Hkv = a->num_kv_heads;
+  P.d = a->head_dim, P.rot = a->rot_dim, P.max_pos = a->max_pos;
+  P.w_dtype = a->w_dtype, P.inter = a->interleaved ? 1u : 0u, P.pos64 = a->pos_i64 ? 1u : 0u;
+  P.eps = a->eps;
+  if (cache) {
+    P.kp = a->k_pool, P.vp = a->v_pool;
+    P.kps = a->kp_page_stride, P.khs = a->kp_head_stride, P.kts = a->kp_tok_stride;
+    P.vps = a->vp_page_stride, P.vhs = a->vp_head_stride, P.vts = a->vp_tok_stride;
+    P.app = a->append_indptr, P.ctx = a->ctx_lens, P.table = a->block_table;
+    P.pind = a->page_indptr, P.ps = a->page_size, P.bt_stride = a->bt_stride;
+    P.num_pages = a->num_pages;
+  }
+  // a grid over (request, token), tokens striding past 65535
+  uint32_t most = cache && a->max_append ? a->max_append : a->num_tokens;
+  if (most > a->num_tokens)
+    most = a->num_tokens;
+  const dim3 grid(cache ? a->num_requests : 1u, most < 65535u ? most : 65535u);
+  auto fn = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
+            : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
+                                        : rotary_rows<SCHED_PD_F16>;
+  hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, static_cast<hipStream_t>(stream), P);
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess)
+    return set_error(-1, "sched_qk_norm_rope: launch failed: %s", hipGetErrorString(e));
+  return 0;
+}
+
+} // extern "C"

@@ -207,7 +207,9 @@ class _Lengths(MutableMapping):
     def __setitem__(self, rid, value):
         if rid not in self._c._slot:
             raise KeyError(f"request {rid!r} not in the cache (add_request first)")
-        self._c._len[self._c._slot[rid]] = int(value)
+        c, slot = self._c, self._c._slot[rid]
+        c._len[slot] = int(value)
+        c._counted[slot] = min(c._counted[slot], c._len[slot])
 
     def __delitem__(self, rid):
         raise TypeError("release(rid) removes a request")
@@ -282,10 +284,14 @@ class PagedKvCache:
       48 / 48;
     - fp32 caches (the VALU kernels) read token-major rows with coalesced
       loads.
-    "dmajor" stays available."""
+    "dmajor" stays available.
+
+    With track_weights, `weights` [P, Hkv, page] float32 holds each token's attention
+    weight, which decode_weighted() adds up and evict() goes by."""
 
     def __init__(self, num_pages: int, num_kv_heads: int, head_dim: int, page_size: int = 16,
-                 dtype=torch.bfloat16, device="cuda", v_layout: str = "auto"):
+                 dtype=torch.bfloat16, device="cuda", v_layout: str = "auto",
+                 track_weights: bool = False):
         self.page_size, self.num_kv_heads, self.head_dim = page_size, num_kv_heads, head_dim
         self.dtype = dtype
         self.device = torch.device(device)
@@ -313,6 +319,11 @@ class PagedKvCache:
         self._free_slots: list = []
         self._len = np.zeros(64, np.int64)
         self._npg = np.zeros(64, np.int64)
+        # tokens evicted so far, and how many of the tokens held have a weight
+        self._cut = np.zeros(64, np.int64)
+        self._counted = np.zeros(64, np.int64)
+        self.weights = torch.zeros(num_pages, num_kv_heads, page_size, dtype=torch.float32,
+                                   device=self.device) if track_weights else None
         self.lens = _Lengths(self)
         self._batch = (None, None)   # (rids as a tuple, their slots): a batch repeats
         self._table = None       # the device block table of the last request list
@@ -328,9 +339,13 @@ class PagedKvCache:
             if slot >= self._len.size:
                 self._len = np.concatenate([self._len, np.zeros_like(self._len)])
                 self._npg = np.concatenate([self._npg, np.zeros_like(self._npg)])
+                self._cut = np.concatenate([self._cut, np.zeros_like(self._cut)])
+                self._counted = np.concatenate([self._counted, np.zeros_like(self._counted)])
         self._slot[rid] = slot
         self._len[slot] = 0
         self._npg[slot] = 0
+        self._cut[slot] = 0
+        self._counted[slot] = 0
         self.pages[rid] = []
         self._batch = (None, None)
 
@@ -358,6 +373,7 @@ class PagedKvCache:
             del pages[keep[i]:]
         self._len[s] = new
         self._npg[s] = np.minimum(self._npg[s], keep)
+        self._counted[s] = np.minimum(self._counted[s], new)
         self._table = None
 
     def _batch_distinct(self) -> bool:
@@ -383,6 +399,12 @@ class PagedKvCache:
         """Tokens each request holds, as an int64 array in rids' order (a
         copy; one gather instead of a lookup per request)."""
         return self._len[self._slots(rids)[1]]
+
+    def positions(self, rids) -> np.ndarray:
+        """Position of each request's next token (int64): the tokens it holds and those
+        evicted from it."""
+        s = self._slots(rids)[1]
+        return self._len[s] + self._cut[s]
 
     def reserve(self, rids, counts) -> None:
         """Allocate pages so that each request has room for counts[i] more
@@ -493,6 +515,37 @@ class PagedKvCache:
     def append(self, rids, k_new, v_new, counts=None, errors=None) -> None:
         """Append counts[i] rows (default 1 each) of k_new / v_new [T, Hkv, d]
         to request rids[i], rows in request order."""
+        self._append(rids, k_new.shape[0], counts, (), lambda app, ctx, bt, most, _: append(
+            k_new, v_new, app, ctx, self.k_pool, self.v_pool, bt, v_layout=self.v_layout,
+            k_scale=self.k_scale, v_scale=self.v_scale, max_append=most, errors=errors))
+
+    def append_rotated(self, rids, q, k_new, v_new, cos_sin, counts=None, positions=None,
+                       stream=None, **kw):
+        """append() of keys that are normed and rotated on their way into the cache, with
+        the queries of the same tokens (rotary.append_rotated, whose keyword arguments
+        these are): q [T, Hq, d], k_new / v_new [T, Hkv, d], rows in request order. Returns
+        the rotated queries. Positions (int32 or int64 [T] on the device) default to the
+        requests' own, which go on counting after an eviction."""
+        import rotary
+        with _on_stream(stream):
+            def launch(app, ctx, bt, most, extra):
+                return rotary.append_rotated(
+                    q, k_new, v_new, positions if positions is not None else extra[0], cos_sin,
+                    app, ctx, self.k_pool, self.v_pool, bt, v_layout=self.v_layout,
+                    k_scale=self.k_scale, v_scale=self.v_scale, max_append=most, **kw)
+
+            def own_positions(s, counts):
+                first = np.repeat(self._len[s] + self._cut[s], counts)
+                return (first + np.arange(first.size)
+                        - np.repeat(np.cumsum(counts) - counts, counts)).astype(np.int32)
+            return self._append(rids, k_new.shape[0], counts,
+                                () if positions is not None else (own_positions,), launch)
+
+    def _append(self, rids, T, counts, extra, launch):
+        """Make room for counts[i] tokens of request rids[i] (T in all), then launch(
+        append_indptr, ctx_lens, block table, largest count, extra arrays): functions of
+        (slots, counts) that are called before the lengths move, uploaded with the
+        lengths. A launch that raises leaves the cache as it was."""
         key, s = self._slots(rids)
         counts = (np.ones(len(key), np.int64) if counts is None
                   else np.asarray([int(c) for c in counts], np.int64))
@@ -500,20 +553,17 @@ class PagedKvCache:
             raise ValueError(f"{counts.size} counts for {len(key)} requests")
         if np.unique(s).size != s.size:
             raise ValueError("a request appears twice in one append")
-        if (counts < 0).any() or int(counts.sum()) != k_new.shape[0]:
-            raise ValueError(f"counts sum to {int(counts.sum())}, sources have "
-                             f"{k_new.shape[0]} rows")
+        if (counts < 0).any() or int(counts.sum()) != T:
+            raise ValueError(f"counts sum to {int(counts.sum())}, sources have {T} rows")
+        extra = tuple(f(s, counts) for f in extra)
         held = self._npg[s].copy()
         self.reserve(key, counts)
         try:
             self._len[s] += counts
             app = np.zeros(len(key) + 1, dtype=np.int32)
             app[1:] = np.cumsum(counts)
-            bt, ctx, (app_dev,) = self._table_step(key, s, (app,))
-            append(k_new, v_new, app_dev, ctx, self.k_pool,
-                   self.v_pool, bt, v_layout=self.v_layout, k_scale=self.k_scale,
-                   v_scale=self.v_scale,
-                   max_append=int(counts.max()) if counts.size else 0, errors=errors)
+            bt, ctx, dev = self._table_step(key, s, (app, *extra))
+            return launch(dev[0], ctx, bt, int(counts.max()) if counts.size else 0, dev[1:])
         except Exception:
             # a rejected launch leaves the cache as it was
             self._len[s] -= counts
@@ -524,6 +574,79 @@ class PagedKvCache:
             self._npg[s] = held
             self._table = None
             raise
+
+    # -- attention weights and eviction ----------------------------------------
+    def _need_weights(self):
+        if self.weights is None:
+            raise ValueError("this cache keeps no weights (track_weights=True)")
+
+    def decode_weighted(self, q, rids, decay=1.0, stream=None, **kw):
+        """decode() that also adds up each token's attention weight in `weights`
+        (decode_maps.paged_decode_weighted, whose keyword arguments these are). Tokens
+        appended since the last call start at this step's weight."""
+        import decode_maps
+        self._need_weights()
+        with _on_stream(stream):
+            key, s = self._slots(rids)
+            if not self._batch_distinct():
+                raise ValueError("a request appears twice in one step")
+            bt, ctx, (counted,) = self._table_step(key, s, (self._counted[s],))
+            out = decode_maps.paged_decode_weighted(
+                q, self.k_pool, self.v_pool, bt, ctx, self.weights, counted=counted, decay=decay,
+                v_layout=self.v_layout, k_scale=self.k_scale, v_scale=self.v_scale, **kw)
+        self._counted[s] = self._len[s]
+        return out
+
+    def decode_diff(self, q, rids, lam, stream=None, **kw):
+        """One differential decode step over the requests' current contexts
+        (decode_maps.paged_decode_diff, whose keyword arguments these are)."""
+        import decode_maps
+        with _on_stream(stream):
+            key, s = self._slots(rids)
+            bt, ctx, _ = self._table_step(key, s)
+            return decode_maps.paged_decode_diff(
+                q, self.k_pool, self.v_pool, bt, ctx, lam, v_layout=self.v_layout,
+                k_scale=self.k_scale, v_scale=self.v_scale, **kw)
+
+    def evict(self, rids, keep, sink=0, recent=0, stream=None, **kw):
+        """Cut each request to at most `keep` tokens (a number, or one per request) by
+        its tokens' weights, per kv-head (eviction.evict, whose result it returns), and free
+        the pages that no longer hold any. `sink` first and `recent` last tokens stay.
+        Tokens without a weight yet (appended since the last decode_weighted()) must be
+        among the recent ones of a request that is cut."""
+        import eviction
+        self._need_weights()
+        key, s = self._slots(rids)
+        if not self._batch_distinct():
+            raise ValueError("a request appears twice in one eviction")
+        n = self._len[s]
+        keep = np.broadcast_to(np.asarray(keep, np.int64), n.shape)
+        if (keep < 0).any():
+            raise ValueError("keep must not be negative")
+        m = np.minimum(n, keep)
+        fresh = n - self._counted[s]
+        late = (m < n) & (fresh > np.minimum(m, recent)) & (m > 0)
+        if late.any():
+            i = int(np.argmax(late))
+            raise ValueError(f"request {key[i]!r} has {int(fresh[i])} tokens without a weight, "
+                             f"more than the {min(int(m[i]), recent)} recent ones kept")
+        with _on_stream(stream):
+            bt, ctx, (m_dev,) = self._table_step(key, s, (m,))
+            kept = eviction.evict(
+                self.k_pool, self.v_pool, self.weights, bt, ctx, m_dev, sink=sink, recent=recent,
+                max_keep=int(m.max()) if m.size else 0, v_layout=self.v_layout,
+                k_scale=self.k_scale, v_scale=self.v_scale, **kw)
+        self._cut[s] += n - m
+        self._counted[s] = np.maximum(0, m - fresh)
+        self._len[s] = m
+        need = -(-m // self.page_size)
+        for i in np.nonzero(need < self._npg[s])[0]:
+            pages = self.pages[key[i]]
+            self.allocator.free(pages[need[i]:])
+            del pages[need[i]:]
+        self._npg[s] = np.minimum(self._npg[s], need)
+        self._table = None
+        return kept
 
     def decode_step(self, q, rids, k_new, v_new, **kw):
         """One serving step: append each request's new token (k_new / v_new

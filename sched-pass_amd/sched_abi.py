@@ -116,6 +116,94 @@ def default_kv_args() -> SchedKvAppendArgs:
     return a
 
 
+# --- decode with attention maps handed on (include/sched_pd.h) -----------------
+MAPS_ABI_VERSION = 1
+MAPS_WEIGHTED, MAPS_DIFF = 0, 1
+
+
+class SchedMapsArgs(ctypes.Structure):
+    """Field-for-field mirror of `SchedMapsArgs` in include/sched_pd.h."""
+    _fields_ = [
+        ("abi_version", _u32), ("op", _u32), ("kv_dtype", _u32), ("q_dtype", _u32),
+        ("o_dtype", _u32), ("num_requests", _u32), ("num_q_heads", _u32),
+        ("num_kv_heads", _u32), ("head_dim", _u32), ("page_size", _u32),
+        ("bt_stride", _u32), ("max_pages", _u32), ("flags", _u32),
+        ("sm_scale", _f32), ("decay", _f32), ("eps", _f32), ("out_scale", _f32),
+        ("num_pages", ctypes.c_uint64),
+        ("q", _p), ("out", _p), ("k_pool", _p), ("v_pool", _p),
+        ("k_page_stride", _i64), ("k_head_stride", _i64), ("k_tok_stride", _i64),
+        ("v_page_stride", _i64), ("v_head_stride", _i64), ("v_tok_stride", _i64),
+        ("v_dim_stride", _i64),
+        ("k_scale", _p), ("v_scale", _p),
+        ("block_table", _p), ("page_indptr", _p), ("ctx_lens", _p),
+        ("weights", _p), ("w_page_stride", _i64), ("w_head_stride", _i64),
+        ("counted", _p), ("lam", _p), ("norm_weight", _p),
+        ("workspace", _p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+# --- query / key norm and rotation, eviction (include/sched_kv.h) --------------
+ROTARY_ABI_VERSION = 1
+EVICT_ABI_VERSION = 1
+
+
+class SchedRotaryArgs(ctypes.Structure):
+    """Field-for-field mirror of `SchedRotaryArgs` in include/sched_kv.h."""
+    _fields_ = [
+        ("abi_version", _u32), ("dtype", _u32), ("w_dtype", _u32), ("num_tokens", _u32),
+        ("num_q_heads", _u32), ("num_kv_heads", _u32), ("head_dim", _u32), ("rot_dim", _u32),
+        ("interleaved", _u32), ("pos_i64", _u32), ("max_pos", _u32), ("eps", _f32),
+        ("q", _p), ("k", _p), ("v", _p),
+        ("q_tok_stride", _i64), ("q_head_stride", _i64), ("k_tok_stride", _i64),
+        ("k_head_stride", _i64), ("v_tok_stride", _i64), ("v_head_stride", _i64),
+        ("q_out", _p), ("k_out", _p),
+        ("qo_tok_stride", _i64), ("qo_head_stride", _i64), ("ko_tok_stride", _i64),
+        ("ko_head_stride", _i64),
+        ("q_weight", _p), ("k_weight", _p), ("positions", _p), ("cos_sin", _p),
+        ("cs_stride", _i64), ("errors", _p),
+        ("num_requests", _u32), ("page_size", _u32), ("bt_stride", _u32), ("max_append", _u32),
+        ("num_pages", ctypes.c_uint64),
+        ("append_indptr", _p), ("ctx_lens", _p), ("block_table", _p), ("page_indptr", _p),
+        ("k_pool", _p), ("v_pool", _p),
+        ("kp_page_stride", _i64), ("kp_head_stride", _i64), ("kp_tok_stride", _i64),
+        ("vp_page_stride", _i64), ("vp_head_stride", _i64), ("vp_tok_stride", _i64),
+    ]
+
+
+class SchedEvictArgs(ctypes.Structure):
+    """Field-for-field mirror of `SchedEvictArgs` in include/sched_kv.h."""
+    _fields_ = [
+        ("abi_version", _u32), ("kv_dtype", _u32), ("num_requests", _u32),
+        ("num_kv_heads", _u32), ("head_dim", _u32), ("page_size", _u32), ("bt_stride", _u32),
+        ("max_pages", _u32), ("max_keep", _u32), ("sink", _u32), ("recent", _u32),
+        ("_pad0", _u32), ("num_pages", ctypes.c_uint64),
+        ("k_pool", _p), ("v_pool", _p),
+        ("k_page_stride", _i64), ("k_head_stride", _i64), ("k_tok_stride", _i64),
+        ("v_page_stride", _i64), ("v_head_stride", _i64), ("v_tok_stride", _i64),
+        ("v_dim_stride", _i64),
+        ("k_scale", _p), ("v_scale", _p), ("weights", _p), ("weights_out", _p),
+        ("w_page_stride", _i64), ("w_head_stride", _i64),
+        ("block_table", _p), ("page_indptr", _p), ("ctx_lens", _p), ("keep_lens", _p),
+        ("kept", _p), ("errors", _p), ("workspace", _p), ("workspace_bytes", ctypes.c_uint64),
+    ]
+
+
+def default_maps_args() -> SchedMapsArgs:
+    """Same defaults as sched_maps_default_args() in C."""
+    return SchedMapsArgs(abi_version=MAPS_ABI_VERSION, kv_dtype=BF16, q_dtype=BF16,
+                         o_dtype=BF16, decay=1.0, eps=1e-5, out_scale=1.0)
+
+
+def default_rotary_args() -> SchedRotaryArgs:
+    """Same defaults as sched_rotary_default_args() in C."""
+    return SchedRotaryArgs(abi_version=ROTARY_ABI_VERSION, dtype=BF16, w_dtype=F32, eps=1e-6)
+
+
+def default_evict_args() -> SchedEvictArgs:
+    """Same defaults as sched_evict_default_args() in C."""
+    return SchedEvictArgs(abi_version=EVICT_ABI_VERSION, kv_dtype=BF16)
+
+
 # Every function include/*.h declares: name -> (restype, argtypes).
 _c_bool = ctypes.c_bool
 SIGNATURES = {
@@ -160,6 +248,15 @@ SIGNATURES = {
     "sched_paged_decode_append": (ctypes.c_int, [ctypes.POINTER(SchedDecodeArgs),
                                                  ctypes.POINTER(SchedKvAppendArgs), _p]),
     "sched_kv_table_update": (ctypes.c_int, [_p, ctypes.c_int64, ctypes.c_int64, _p, _u32, _p]),
+    "sched_maps_default_args": (None, [ctypes.POINTER(SchedMapsArgs)]),
+    "sched_decode_maps": (ctypes.c_int, [ctypes.POINTER(SchedMapsArgs), _p]),
+    "sched_decode_maps_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SchedMapsArgs)]),
+    "sched_decode_maps_kernel_kind": (ctypes.c_int, [ctypes.POINTER(SchedMapsArgs)]),
+    "sched_rotary_default_args": (None, [ctypes.POINTER(SchedRotaryArgs)]),
+    "sched_qk_norm_rope": (ctypes.c_int, [ctypes.POINTER(SchedRotaryArgs), _p]),
+    "sched_evict_default_args": (None, [ctypes.POINTER(SchedEvictArgs)]),
+    "sched_kv_evict": (ctypes.c_int, [ctypes.POINTER(SchedEvictArgs), _p]),
+    "sched_kv_evict_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(SchedEvictArgs)]),
     "launch_paged_softmax": (None, [_p, _p, _p, _p, _p, ctypes.c_int, ctypes.c_int,
                                     ctypes.c_int, _p]),
     "paged_softmax_occupancy": (ctypes.c_int, []),
