@@ -9,7 +9,7 @@
 #include <cmath>
 #include <cstdint>
 
-#include "maps.h"
+#include "maps_mfma.h"
 #include "rt_internal.h"
 
 using namespace schedpd;
@@ -43,7 +43,8 @@ __global__ void __launch_bounds__(kBlock) maps_valu(MapParams P) {
   __shared__ float s_c[kMostRows];
   __shared__ int32_t s_page[TT / 4];
   const uint32_t tid = threadIdx.x, lane32 = tid & 31u, grp = tid >> 5;
-  const uint32_t item = blockIdx.x, task = item / P.nsplit, chunk = item % P.nsplit;
+  const uint32_t task = blockIdx.x, chunk = blockIdx.y;
+  const uint64_t item = (uint64_t)task * P.nsplit + chunk;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
   const uint64_t first = (uint64_t)chunk * len;
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(kBlock) maps_valu(MapParams P) {
   for (uint32_t k = 0; k < 2; ++k) {
     const uint32_t g = grp + 8u * k;
     if (g < P.rows && lane32 == 0) {
-      float *ml = P.ml + ((uint64_t)item * P.rows + g) * 2u;
+      float *ml = P.ml + (item * P.rows + g) * 2u;
       ml[0] = m[k];
       ml[1] = l[k];
     }
@@ -162,11 +163,12 @@ __global__ void __launch_bounds__(kBlock) maps_valu(MapParams P) {
   for (uint32_t i = 0; i < RPL; ++i) {
     const uint32_t g = rg + RG * i;
     if (g < P.rows)
-      P.acc[((uint64_t)item * P.rows + g) * D + j0] = acc[i];
+      P.acc[(item * P.rows + g) * D + j0] = acc[i];
   }
 }
 
-// The join: workgroup (task, b). b = 0 writes the task's outputs; the weights' token
+// The join of what `maps_valu` and, for tasks of several chunks, maps_mfma left:
+// workgroup (task, b). b = 0 writes the task's outputs; the weights' token
 // blocks are dealt out over all b.
 template <bool DIFF> __global__ void __launch_bounds__(kBlock) maps_join(MapParams P) {
   __shared__ float s_m[kMostRows], s_li[kMostRows], s_sum[kBlock / 64];
@@ -174,6 +176,8 @@ template <bool DIFF> __global__ void __launch_bounds__(kBlock) maps_join(MapPara
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
   const uint32_t nch = n == 0u ? 1u : (n + len - 1u) / len;
+  if (nch <= P.join_from)
+    return; // the stream has finished this task
   const uint64_t item0 = (uint64_t)task * P.nsplit;
   if (tid < P.rows) {
     const float *ml = P.ml + (item0 * P.rows + tid) * 2u;
@@ -254,6 +258,7 @@ uint64_t elem_bytes(uint32_t dt) {
 
 // What a call's shape decides: how far tasks are split, and the workspace.
 struct Plan {
+  bool mfma;
   uint32_t rows, nsplit, least;
   uint64_t score_blocks, ml_off, acc_off, total;
 };
@@ -297,25 +302,56 @@ int check_shape(const SchedMapsArgs *a) {
     return set_error(hipErrorInvalidValue, "sched_decode_maps: num_pages %llu",
                      (unsigned long long)a->num_pages);
   if ((uint64_t)a->num_requests * a->num_kv_heads > (1u << 24) ||
-      (uint64_t)a->max_pages * a->page_size > 0x7fffffffull)
+      (uint64_t)a->max_pages * a->page_size > (1u << 24))
     return set_error(hipErrorInvalidValue, "sched_decode_maps: %u requests x %u kv-heads, tables "
                                            "of %u pages", a->num_requests, a->num_kv_heads,
                      a->max_pages);
   return 0;
 }
 
-// Chunks fill the card this many times over; none is shorter than kLeastTokens.
+// The matrix cores: 16-bit caches with queries of their type, fp8 ones with bf16
+// queries, rows that 16-byte loads reach, and lane offsets within 32 bits.
+bool mfma_applies(const SchedMapsArgs *a) {
+  if ((a->flags & SCHED_PD_FLAG_FORCE_VALU) || a->kv_dtype == SCHED_PD_F32 || a->head_dim == 32)
+    return false;
+  const bool fp8 = a->kv_dtype == SCHED_PD_FP8_E4M3;
+  if (a->q_dtype != (fp8 ? SCHED_PD_BF16 : a->kv_dtype))
+    return false;
+  const int64_t eb = fp8 ? 1 : 2;
+  const bool vt = a->v_dim_stride == 1;
+  const int64_t vrow = (vt ? a->v_tok_stride : a->v_dim_stride) * eb, krow = a->k_tok_stride * eb;
+  for (int64_t s : {a->k_page_stride * eb, a->k_head_stride * eb, krow, a->v_page_stride * eb,
+                    a->v_head_stride * eb, vrow})
+    if (s % 16)
+      return false;
+  return krow > 0 && vrow > 0 && krow < (1 << 26) && vrow < (1 << 25) &&
+         ((uintptr_t)a->k_pool & 15u) == 0 && ((uintptr_t)a->v_pool & 15u) == 0 &&
+         ((uintptr_t)a->q & 15u) == 0;
+}
+
+// Chunks fill the card this many times over; none is shorter than kLeastTokens. A weighted
+// chunk's scores fit kScoreBytes of LDS on the matrix cores.
 constexpr uint32_t kItems = 1024, kLeastTokens = 256, kMostSplit = 64;
+constexpr uint32_t kScoreBytes = 32u << 10;
 
 Plan plan_of(const SchedMapsArgs *a) {
   Plan p{};
   const uint64_t tasks = std::max<uint64_t>(1, (uint64_t)a->num_requests * a->num_kv_heads);
   const uint64_t longest = (uint64_t)a->max_pages * a->page_size;
-  p.rows = a->num_q_heads / a->num_kv_heads * (a->op == SCHED_MAPS_DIFF ? 2u : 1u);
+  const bool weighted = a->op == SCHED_MAPS_WEIGHTED;
+  p.mfma = mfma_applies(a);
+  p.rows = a->num_q_heads / a->num_kv_heads * (weighted ? 1u : 2u);
   p.least = kLeastTokens;
-  const uint64_t want = (kItems + tasks - 1) / tasks, can = (longest + p.least - 1) / p.least;
-  p.nsplit = (uint32_t)std::max<uint64_t>(1, std::min<uint64_t>({want, can, kMostSplit}));
-  if (a->op == SCHED_MAPS_WEIGHTED) {
+  uint64_t want = (kItems + tasks - 1) / tasks;
+  const uint64_t can = (longest + p.least - 1) / p.least;
+  want = std::min<uint64_t>({want, can, kMostSplit});
+  if (weighted && p.mfma) {
+    // map_chunk rounds up to 64 tokens
+    const uint64_t fits = kScoreBytes / (p.rows * 4u) - 63u;
+    want = std::max<uint64_t>(want, (longest + fits - 1) / fits);
+  }
+  p.nsplit = (uint32_t)std::max<uint64_t>(1, want);
+  if (weighted) {
     // a call's pages are distinct: never more of them than the pool has
     uint64_t pages = a->page_indptr ? a->max_pages : (uint64_t)a->num_requests * a->max_pages;
     pages = std::min<uint64_t>(pages, a->num_pages);
@@ -336,6 +372,36 @@ template <typename T> StreamFn valu_of(uint32_t d, bool diff) {
   case 128: return diff ? maps_valu<T, 128, true> : maps_valu<T, 128, false>;
   default: return diff ? maps_valu<T, 256, true> : maps_valu<T, 256, false>;
   }
+}
+
+// Blocks in flight per wave and waves per SIMD they leave room for.
+template <int KV, int D, bool VT, bool DIFF> StreamFn mfma_rows(uint32_t rows) {
+#ifndef D256
+#define D256 1
+#endif
+#ifndef W256
+#define W256 2
+#endif
+#ifndef W128
+#define W128 3
+#endif
+  constexpr int DEPTH = D == 256 ? (KV == kMapFp8 ? 2 : D256) : D == 128 ? (KV == kMapFp8 ? 3 : 2) : 4;
+  constexpr int WPE = D == 256 ? W256 : D == 128 ? W128 : 3;
+  return rows <= 4   ? maps_mfma<KV, D, VT, 4, DIFF, 4, DEPTH, WPE>
+         : rows <= 8 ? maps_mfma<KV, D, VT, 8, DIFF, 4, DEPTH, WPE>
+                     : maps_mfma<KV, D, VT, 16, DIFF, 4, DEPTH, WPE>;
+}
+
+template <int KV, bool VT> StreamFn mfma_of(uint32_t d, bool diff, uint32_t rows) {
+  if (d == 64)
+    return diff ? mfma_rows<KV, 64, VT, true>(rows) : mfma_rows<KV, 64, VT, false>(rows);
+  if (d == 128)
+    return diff ? mfma_rows<KV, 128, VT, true>(rows) : mfma_rows<KV, 128, VT, false>(rows);
+  return diff ? mfma_rows<KV, 256, VT, true>(rows) : mfma_rows<KV, 256, VT, false>(rows);
+}
+
+template <int KV> StreamFn mfma_of(uint32_t d, bool vt, bool diff, uint32_t rows) {
+  return vt ? mfma_of<KV, true>(d, diff, rows) : mfma_of<KV, false>(d, diff, rows);
 }
 
 } // namespace
@@ -362,7 +428,7 @@ int64_t sched_decode_maps_workspace_bytes(const SchedMapsArgs *a) {
 int sched_decode_maps_kernel_kind(const SchedMapsArgs *a) {
   if (check_shape(a))
     return -1;
-  return 0;
+  return mfma_applies(a) ? 1 : 0;
 }
 
 int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
@@ -420,21 +486,34 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   P.ml = reinterpret_cast<float *>(ws + plan.ml_off);
   P.acc = reinterpret_cast<float *>(ws + plan.acc_off);
 
+  P.join_from = plan.mfma ? 1u : 0u;
   const uint32_t tasks = P.R * P.Hkv;
-  StreamFn fn = a->kv_dtype == SCHED_PD_F32    ? valu_of<float>(P.D, diff)
-                : a->kv_dtype == SCHED_PD_BF16 ? valu_of<uint16_t>(P.D, diff)
-                : a->kv_dtype == SCHED_PD_F16  ? valu_of<_Float16>(P.D, diff)
-                                               : valu_of<uint8_t>(P.D, diff);
+  StreamFn fn;
+  if (plan.mfma)
+    fn = a->kv_dtype == SCHED_PD_BF16  ? mfma_of<kMapBf16>(P.D, P.vds == 1, diff, P.rows)
+         : a->kv_dtype == SCHED_PD_F16 ? mfma_of<kMapF16>(P.D, P.vds == 1, diff, P.rows)
+                                       : mfma_of<kMapFp8>(P.D, P.vds == 1, diff, P.rows);
+  else
+    fn = a->kv_dtype == SCHED_PD_F32    ? valu_of<float>(P.D, diff)
+         : a->kv_dtype == SCHED_PD_BF16 ? valu_of<uint16_t>(P.D, diff)
+         : a->kv_dtype == SCHED_PD_F16  ? valu_of<_Float16>(P.D, diff)
+                                        : valu_of<uint8_t>(P.D, diff);
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(fn, dim3(tasks * P.nsplit), dim3(kBlock), 0, s, P);
+  const uint64_t longest = (uint64_t)P.max_pages * P.ps;
+  uint32_t lds = 0;
+  if (plan.mfma && !diff) {
+    // the longest chunk's scores
+    const uint64_t even = (longest + P.nsplit - 1) / P.nsplit;
+    const uint64_t chunk = (std::max<uint64_t>(std::min<uint64_t>(even, longest), P.least) + 63) & ~uint64_t(63);
+    lds = (uint32_t)(chunk * P.rows * 4u);
+  }
+  hipLaunchKernelGGL(fn, dim3(tasks, P.nsplit), dim3(kBlock), lds, s, P);
   hipError_t e = hipGetLastError();
-  if (e == hipSuccess) {
+  if (e == hipSuccess && P.nsplit > P.join_from) {
     uint32_t by = 1;
-    if (!diff) {
-      const uint64_t longest = (uint64_t)P.max_pages * P.ps;
+    if (!diff)
       by = (uint32_t)std::max<uint64_t>(
           1, std::min<uint64_t>((longest + 4 * kBlock - 1) / (4 * kBlock), 4096u / tasks + 1u));
-    }
     hipLaunchKernelGGL(diff ? maps_join<true> : maps_join<false>, dim3(tasks, by), dim3(kBlock), 0,
                        s, P);
     e = hipGetLastError();

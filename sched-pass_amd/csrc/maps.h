@@ -29,6 +29,7 @@ struct MapParams {
   uint32_t D, ps, bt_stride, max_pages, num_pages;
   uint32_t q_dtype, o_dtype;
   uint32_t nsplit, least; // most chunks of a task; least tokens of one (a multiple of 64)
+  uint32_t join_from;     // the join has tasks of more chunks than this to do
   float scale_log2;
   // weighted
   float *w;
