@@ -167,11 +167,44 @@ __global__ void __launch_bounds__(kBlock) maps_valu(MapParams P) {
   }
 }
 
+constexpr int kJoin = 512;
+
+// Rows [g0, g1) of a task joined over its chunks: M and 1 / L into s_M, s_Li. A wave
+// takes a row at a time, its lanes the chunks.
+__device__ __forceinline__ void join_rows(const MapParams &P, uint64_t item0, uint32_t nch,
+                                          uint32_t g0, uint32_t g1, float *s_M, float *s_Li) {
+  const uint32_t lane = threadIdx.x & 63u;
+  for (uint32_t g = g0 + (threadIdx.x >> 6); g < g1; g += kJoin / 64) {
+    float m = kMInit, l = 0.f;
+    for (uint32_t c = lane; c < nch; c += 64u) {
+      const float *e = P.ml + ((item0 + c) * P.rows + g) * 2u;
+      const float mc = e[0], lc = e[1], mn = fmaxf(m, mc);
+      l = l * __builtin_amdgcn_exp2f(m - mn) + lc * __builtin_amdgcn_exp2f(mc - mn);
+      m = mn;
+    }
+    float M = m;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+      M = fmaxf(M, __shfl_xor(M, o));
+    float L = l * __builtin_amdgcn_exp2f(m - M);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1)
+      L += __shfl_xor(L, o);
+    if (lane == 0) {
+      s_M[g] = M;
+      s_Li[g] = 1.f / L;
+    }
+  }
+}
+
 // The join of what `maps_valu` and, for tasks of several chunks, maps_mfma left:
-// workgroup (task, b). b = 0 writes the task's outputs; the weights' token
-// blocks are dealt out over all b.
-template <bool DIFF> __global__ void __launch_bounds__(kBlock) maps_join(MapParams P) {
-  __shared__ float s_m[kMostRows], s_li[kMostRows], s_sum[kBlock / 64];
+// workgroup (task, y). y < G: q-head y's output; from there on the weights, their tokens dealt
+// out over the workgroups. A dim's chunks are summed by kJoin / D lanes, 8 loads in flight
+// each, and their sums in order.
+template <int D, bool DIFF> __global__ void __launch_bounds__(kJoin) maps_join(MapParams P) {
+  constexpr uint32_t LANES = kJoin / D, NR = DIFF ? 2 : 1, CH = 64;
+  __shared__ float s_M[kMostRows], s_Li[kMostRows];
+  __shared__ float s_f[NR][CH], s_o[NR][LANES][D], s_sum[kJoin / 64];
   const uint32_t tid = threadIdx.x, task = blockIdx.x;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
@@ -179,75 +212,110 @@ template <bool DIFF> __global__ void __launch_bounds__(kBlock) maps_join(MapPara
   if (nch <= P.join_from)
     return; // the stream has finished this task
   const uint64_t item0 = (uint64_t)task * P.nsplit;
-  if (tid < P.rows) {
-    const float *ml = P.ml + (item0 * P.rows + tid) * 2u;
-    float M = ml[0];
-    for (uint32_t c = 1; c < nch; ++c)
-      M = fmaxf(M, ml[(uint64_t)c * P.rows * 2u]);
-    float L = 0.f;
-    for (uint32_t c = 0; c < nch; ++c) {
-      const float *e = ml + (uint64_t)c * P.rows * 2u;
-      L += e[1] * __builtin_amdgcn_exp2f(e[0] - M);
-    }
-    s_m[tid] = M;
-    s_li[tid] = 1.f / L;
-  }
-  __syncthreads();
-  if (blockIdx.y == 0) {
-    const uint32_t D = P.D;
-    auto joined = [&](uint32_t g, uint32_t j) {
-      float o = 0.f;
-      for (uint32_t c = 0; c < nch; ++c) {
-        const uint64_t e = (item0 + c) * P.rows + g;
-        o += P.acc[e * D + j] * __builtin_amdgcn_exp2f(P.ml[e * 2u] - s_m[g]);
+  if (blockIdx.y < P.G) {
+    const uint32_t g = blockIdx.y, g0 = g * NR, hq = h * P.G + g;
+    join_rows(P, item0, nch, g0, g0 + NR, s_M, s_Li);
+    const uint32_t j = tid % D, part = tid / D;
+    float o[NR] = {};
+    for (uint32_t c0 = 0; c0 < nch; c0 += CH) {
+      const uint32_t cnt = min(CH, nch - c0);
+      __syncthreads(); // the rows are joined; the previous shares have been used
+      if (tid < NR * CH) {
+        const uint32_t k = tid / CH, c = tid % CH;
+        s_f[k][c] = c < cnt ? __builtin_amdgcn_exp2f(P.ml[((item0 + c0 + c) * P.rows + g0 + k) * 2u] -
+                                                     s_M[g0 + k]) * s_Li[g0 + k]
+                            : 0.f;
       }
-      return o * s_li[g];
-    };
-    if constexpr (!DIFF) {
-      for (uint32_t i = tid; i < P.G * D; i += kBlock)
-        map_store(P, ((int64_t)r * P.Hq + h * P.G + i / D) * D + i % D, n ? joined(i / D, i % D)
-                                                                         : __builtin_nanf(""));
-    } else {
-      for (uint32_t g = 0; g < P.G; ++g) {
-        const uint32_t hq = h * P.G + g;
-        float o = 0.f;
-        if (tid < D)
-          o = joined(2u * g, tid) - P.lam[hq] * joined(2u * g + 1u, tid);
-        float inv = 1.f;
-        if (P.nw) {
-          float ss = o * o;
+      __syncthreads();
+      for (uint32_t c = part; c < cnt; c += 8u * LANES) {
+        float v[8][NR];
 #pragma unroll
-          for (int k = 32; k > 0; k >>= 1)
-            ss += __shfl_xor(ss, k);
-          __syncthreads(); // the previous head's sums have been read
-          if ((tid & 63u) == 0u)
-            s_sum[tid >> 6] = ss;
-          __syncthreads();
-          ss = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
-          inv = rsqrtf(ss / (float)D + P.eps);
+        for (uint32_t u = 0; u < 8; ++u) {
+          const uint32_t cc = min(c + u * LANES, cnt - 1u);
+#pragma unroll
+          for (uint32_t k = 0; k < NR; ++k)
+            v[u][k] = P.acc[((item0 + c0 + cc) * P.rows + g0 + k) * D + j];
         }
-        if (tid < D)
-          map_store(P, ((int64_t)r * P.Hq + hq) * D + tid,
-                    n ? o * inv * (P.nw ? P.nw[tid] : 1.f) * P.mul : __builtin_nanf(""));
+#pragma unroll
+        for (uint32_t u = 0; u < 8; ++u)
+#pragma unroll
+          for (uint32_t k = 0; k < NR; ++k)
+            if (c + u * LANES < cnt)
+              o[k] += v[u][k] * s_f[k][c + u * LANES];
       }
     }
+#pragma unroll
+    for (uint32_t k = 0; k < NR; ++k)
+      s_o[k][part][j] = o[k];
+    __syncthreads();
+    float x = 0.f;
+    if (tid < D) {
+      float t[NR];
+#pragma unroll
+      for (uint32_t k = 0; k < NR; ++k) {
+        t[k] = s_o[k][0][tid];
+#pragma unroll
+        for (uint32_t q = 1; q < LANES; ++q)
+          t[k] += s_o[k][q][tid];
+      }
+      x = t[0];
+      if constexpr (DIFF)
+        x -= P.lam[hq] * t[NR - 1];
+    }
+    if constexpr (DIFF) {
+      float inv = P.mul;
+      if (P.nw) {
+        float ss = x * x;
+#pragma unroll
+        for (int k = 32; k > 0; k >>= 1)
+          ss += __shfl_xor(ss, k);
+        if ((tid & 63u) == 0u)
+          s_sum[tid >> 6] = ss;
+        __syncthreads();
+        ss = s_sum[0];
+#pragma unroll
+        for (int k = 1; k < D / 64; ++k)
+          ss += s_sum[k];
+        inv *= rsqrtf(ss / (float)D + P.eps);
+        if (tid < D)
+          inv *= P.nw[tid];
+      }
+      x *= inv;
+    }
+    if (tid < D)
+      map_store(P, ((int64_t)r * P.Hq + hq) * D + tid, n ? x : __builtin_nanf(""));
+    return;
   }
   if constexpr (!DIFF) {
+    const uint32_t first = (blockIdx.y - P.G) * kJoin, stride = (gridDim.y - P.G) * kJoin;
+    if (first >= n)
+      return;
+    join_rows(P, item0, nch, 0u, P.rows, s_M, s_Li);
     const uint64_t b0 = blocks_before(P, r);
     const int64_t row = map_row(P, r);
-    const int64_t cnt = P.counted ? (int64_t)P.counted[r] : (int64_t)n;
-    for (uint32_t t = blockIdx.y * kBlock + tid; t < n; t += gridDim.y * kBlock) {
+    const int64_t have = P.counted ? (int64_t)P.counted[r] : (int64_t)n;
+    __syncthreads();
+    for (uint32_t t = first + tid; t < n; t += stride) {
       const uint32_t page = (uint32_t)P.bt[row + t / P.ps];
       if (page >= P.num_pages || b0 + t / 16u >= P.score_blocks)
         continue;
       const float *s = score_block(P, b0, t / 16u, h) + (t & 15u);
       float *w = P.w + (int64_t)page * P.w_ps + (int64_t)h * P.w_hs + t % P.ps;
+      const float old = (int64_t)t < have ? *w * P.decay : 0.f;
       float a = 0.f;
+#pragma unroll 4
       for (uint32_t g = 0; g < P.rows; ++g)
-        a += __builtin_amdgcn_exp2f(s[g * 16u] - s_m[g]) * s_li[g];
-      *w = (int64_t)t < cnt ? *w * P.decay + a : a;
+        a += __builtin_amdgcn_exp2f(s[g * 16u] - s_M[g]) * s_Li[g];
+      *w = old + a;
     }
   }
+}
+
+template <bool DIFF> auto join_of(uint32_t d) {
+  return d == 32    ? maps_join<DIFF ? 64 : 32, DIFF>
+         : d == 64  ? maps_join<64, DIFF>
+         : d == 128 ? maps_join<128, DIFF>
+                    : maps_join<256, DIFF>;
 }
 
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
@@ -331,8 +399,17 @@ bool mfma_applies(const SchedMapsArgs *a) {
 
 // Chunks fill the card this many times over; none is shorter than kLeastTokens. A weighted
 // chunk's scores fit kScoreBytes of LDS on the matrix cores.
-constexpr uint32_t kItems = 1024, kLeastTokens = 256, kMostSplit = 64;
-constexpr uint32_t kScoreBytes = 32u << 10;
+#ifndef ITEMS
+#define ITEMS 1024
+#endif
+#ifndef LEAST
+#define LEAST 256
+#endif
+#ifndef SCB
+#define SCB 40
+#endif
+constexpr uint32_t kItems = ITEMS, kLeastTokens = LEAST, kMostSplit = 64;
+constexpr uint32_t kScoreBytes = SCB << 10;
 
 Plan plan_of(const SchedMapsArgs *a) {
   Plan p{};
@@ -346,8 +423,7 @@ Plan plan_of(const SchedMapsArgs *a) {
   const uint64_t can = (longest + p.least - 1) / p.least;
   want = std::min<uint64_t>({want, can, kMostSplit});
   if (weighted && p.mfma) {
-    // map_chunk rounds up to 64 tokens
-    const uint64_t fits = kScoreBytes / (p.rows * 4u) - 63u;
+    const uint64_t fits = kScoreBytes / (p.rows * 4u) / 64u * 64u; // (chunks are 64s of tokens)
     want = std::max<uint64_t>(want, (longest + fits - 1) / fits);
   }
   p.nsplit = (uint32_t)std::max<uint64_t>(1, want);
@@ -510,12 +586,12 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   hipLaunchKernelGGL(fn, dim3(tasks, P.nsplit), dim3(kBlock), lds, s, P);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && P.nsplit > P.join_from) {
-    uint32_t by = 1;
-    if (!diff)
-      by = (uint32_t)std::max<uint64_t>(
-          1, std::min<uint64_t>((longest + 4 * kBlock - 1) / (4 * kBlock), 4096u / tasks + 1u));
-    hipLaunchKernelGGL(diff ? maps_join<true> : maps_join<false>, dim3(tasks, by), dim3(kBlock), 0,
-                       s, P);
+    uint32_t by = P.G;
+    if (!diff) // two tokens a lane, fewer workgroups where the tasks are many
+      by += (uint32_t)std::max<uint64_t>(
+          1, std::min<uint64_t>((longest + 2 * kJoin - 1) / (2 * kJoin), 4096u / tasks + 1u));
+    hipLaunchKernelGGL(diff ? join_of<true>(P.D) : join_of<false>(P.D), dim3(tasks, by),
+                       dim3(kJoin), 0, s, P);
     e = hipGetLastError();
   }
   if (e != hipSuccess)

@@ -21,6 +21,11 @@ using namespace schedpd;
 namespace {
 
 constexpr int kBlock = 256;
+#ifndef MANYT
+#define MANYT 1024
+#endif
+// From this many tokens on a workgroup takes four rounds of a token's rows, below one.
+constexpr uint32_t kManyTokens = MANYT;
 
 struct RParams {
   const void *q, *k, *v;
@@ -195,6 +200,187 @@ template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams 
   }
 }
 
+typedef __attribute__((ext_vector_type(4))) unsigned u32x4_t;
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+
+template <int DT, int V> __device__ __forceinline__ void unpack(const u32x4_t &r, float x[V]) {
+  if constexpr (DT == SCHED_PD_F32) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      x[i] = __uint_as_float(r[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const unsigned w = r[i];
+      if constexpr (DT == SCHED_PD_BF16) {
+        x[2 * i] = __uint_as_float(w << 16);
+        x[2 * i + 1] = __uint_as_float(w & 0xffff0000u);
+      } else {
+        const f16x2_t h = __builtin_bit_cast(f16x2_t, w);
+        x[2 * i] = (float)h.x;
+        x[2 * i + 1] = (float)h.y;
+      }
+    }
+  }
+}
+
+template <int DT, int V> __device__ __forceinline__ u32x4_t pack(const float x[V]) {
+  u32x4_t r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (DT == SCHED_PD_F32)
+      r[i] = __float_as_uint(x[i]);
+    else
+      r[i] = DT == SCHED_PD_BF16 ? pack_bf16_rne(x[2 * i], x[2 * i + 1])
+                                 : pack_f16_rne(x[2 * i], x[2 * i + 1]);
+  }
+  return r;
+}
+
+// N (2, 4 or 8) floats at p, 16-byte aligned (8-byte for two).
+template <int N> __device__ __forceinline__ void load_f32(const float *p, float *x) {
+  if constexpr (N == 2) {
+    typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+    const f32x2_t v = *reinterpret_cast<const f32x2_t *>(p);
+    x[0] = v.x, x[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const f32x4_t v = *reinterpret_cast<const f32x4_t *>(p + 4 * i);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        x[4 * i + k] = v[k];
+    }
+  }
+}
+
+// Rows that 16-byte loads reach: L = d / V lanes hold a row (V elements each, L a power
+// of two), so a wave holds 64 / L rows and no lane is idle; the sum of squares and the
+// exchange of the pairs' halves stay within a row's lanes. A workgroup takes U * (256 / L)
+// rows of one token, all their loads in flight together; a lane's angles and weights
+// are those of its dims, loaded once for all of them.
+template <int DT, bool INTER, int U>
+__global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, uint32_t lg) {
+  constexpr int V = DT == SCHED_PD_F32 ? 4 : 8; // elements of a lane
+  const uint32_t tid = threadIdx.x, L = 1u << lg, li = tid & (L - 1u), grp = tid >> lg;
+  const uint32_t groups = kBlock >> lg, d0 = li * V, half = P.rot / 2u;
+  const Span S = span_of(P, blockIdx.x);
+  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), row0 = blockIdx.z * groups * U + grp;
+  const bool turned = d0 < P.rot, first = INTER || d0 < half;
+  // the lane that holds the other halves of this lane's pairs
+  const uint32_t hl = half / V;
+  const int mate = INTER || !turned ? (int)tid : (int)(first ? tid + hl : tid - hl);
+  const bool has_q = P.qw != nullptr, has_k = P.kw != nullptr;
+  float wq[V], wk[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    wq[e] = wk[e] = 1.f;
+  if (blockIdx.y < S.n) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      if (has_q)
+        wq[e] = load_w(P, P.qw, d0 + e);
+      if (has_k)
+        wk[e] = load_w(P, P.kw, d0 + e);
+    }
+  }
+  for (int64_t i = blockIdx.y; i < S.n; i += gridDim.y) {
+    const int64_t tok = S.a0 + i;
+    const int64_t pos = position_of(P, tok);
+    u32x4_t raw[U];
+    const char *src[U];
+    char *dst[U];
+    Place at{-1, 0};
+    if (P.kp)
+      at = place_of(P, S, i);
+    const bool bad = pos < 0 || pos >= (int64_t)P.max_pos;
+    if (blockIdx.z == 0 && tid == 0 && P.errors) {
+      if (bad)
+        atomicAdd(P.errors, 1u);
+      else if (P.kp && at.page < 0)
+        atomicAdd(P.errors, P.Hkv);
+    }
+    if (bad)
+      continue;
+    constexpr int EB = DT == SCHED_PD_F32 ? 4 : 2;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t row = row0 + u * groups;
+      const bool isq = row < P.Hq, isk = !isq && row < P.Hq + P.Hkv;
+      const uint32_t h = isq ? row : isk ? row - P.Hq : row - P.Hq - P.Hkv;
+      const char *base = static_cast<const char *>(isq ? P.q : isk ? P.k : P.v);
+      const int64_t off = isq   ? tok * P.q_ts + h * P.q_hs
+                          : isk ? tok * P.k_ts + h * P.k_hs
+                                : tok * P.v_ts + h * P.v_hs;
+      src[u] = row < rows ? base + (off + d0) * EB : nullptr;
+      char *to = nullptr;
+      if (isq)
+        to = static_cast<char *>(P.qo) + (tok * P.qo_ts + h * P.qo_hs + d0) * EB;
+      else if (P.kp == nullptr)
+        to = static_cast<char *>(P.ko) + (tok * P.ko_ts + h * P.ko_hs + d0) * EB;
+      else if (at.page >= 0)
+        to = isk ? static_cast<char *>(P.kp) +
+                       (at.page * P.kps + h * P.khs + at.slot * P.kts + d0) * EB
+                 : static_cast<char *>(P.vp) +
+                       (at.page * P.vps + h * P.vhs + at.slot * P.vts + d0) * EB;
+      dst[u] = row < rows ? to : nullptr;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (src[u] != nullptr)
+        raw[u] = *reinterpret_cast<const u32x4_t *>(src[u]);
+    constexpr int NC = INTER ? V / 2 : V;
+    float c[NC], sn[NC];
+    if (turned) {
+      const float *cs = P.cs + pos * P.cs_stride + (INTER ? d0 / 2 : first ? d0 : d0 - half);
+      load_f32<NC>(cs, c);
+      load_f32<NC>(cs + half, sn);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t row = row0 + u * groups;
+      const bool isq = row < P.Hq, isv = row >= P.Hq + P.Hkv;
+      float x[V];
+      unpack<DT, V>(raw[u], x);
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        ss += x[e] * x[e];
+      for (uint32_t o = L / 2u; o > 0u; o >>= 1)
+        ss += __shfl_xor(ss, (int)o);
+      const bool norm = isq ? has_q : has_k;
+      const float inv = norm ? rsqrtf(ss / (float)P.d + P.eps) : 1.f;
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        x[e] *= inv * (isq ? wq[e] : wk[e]);
+      float y[V];
+      if constexpr (INTER) {
+#pragma unroll
+        for (int e = 0; e < V; e += 2) {
+          y[e] = x[e] * c[e / 2] - x[e + 1] * sn[e / 2];
+          y[e + 1] = x[e + 1] * c[e / 2] + x[e] * sn[e / 2];
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          const float b = __shfl(x[e], mate);
+          y[e] = first ? x[e] * c[e] - b * sn[e] : x[e] * c[e] + b * sn[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        y[e] = turned ? y[e] : x[e];
+      if (dst[u] != nullptr)
+        *reinterpret_cast<u32x4_t *>(dst[u]) = isv ? raw[u] : pack<DT, V>(y);
+    }
+  }
+}
+
+template <int DT> auto vec_kernel(bool inter, bool many) {
+  return inter ? (many ? rotary_vec<DT, true, 4> : rotary_vec<DT, true, 1>)
+               : (many ? rotary_vec<DT, false, 4> : rotary_vec<DT, false, 1>);
+}
+
 uint32_t esize(uint32_t dt) { return dt == SCHED_PD_F32 ? 4u : 2u; }
 
 bool is_float(uint32_t dt) {
@@ -291,11 +477,43 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
   uint32_t most = cache && a->max_append ? a->max_append : a->num_tokens;
   if (most > a->num_tokens)
     most = a->num_tokens;
-  const dim3 grid(cache ? a->num_requests : 1u, most < 65535u ? most : 65535u);
-  auto fn = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
-            : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
-                                        : rotary_rows<SCHED_PD_F16>;
-  hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, static_cast<hipStream_t>(stream), P);
+  dim3 grid(cache ? a->num_requests : 1u, most < 65535u ? most : 65535u);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  // 16-byte pieces: whole in each row, aligned everywhere, pairs' halves in whole pieces
+  const uint32_t v = 16u / es, lanes = a->head_dim / v;
+  auto pieces = [&](int64_t x) { return x % v == 0; };
+  bool vec = a->head_dim % v == 0 && lanes >= 1 && lanes <= 64 && (lanes & (lanes - 1u)) == 0 &&
+             pieces(P.q_ts) && pieces(P.q_hs) && pieces(P.k_ts) && pieces(P.k_hs) &&
+             pieces(P.qo_ts) && pieces(P.qo_hs) && a->rot_dim % v == 0 &&
+             (P.inter || (a->rot_dim / 2u) % v == 0) && a->cs_stride % 4 == 0 &&
+             (uintptr_t)a->cos_sin % 16 == 0 && (a->rot_dim / 2u) % 4 == 0;
+  if (cache)
+    vec = vec && pieces(P.v_ts) && pieces(P.v_hs) && pieces(P.kps) && pieces(P.khs) &&
+          pieces(P.kts) && pieces(P.vps) && pieces(P.vhs) && pieces(P.vts);
+  else
+    vec = vec && pieces(P.ko_ts) && pieces(P.ko_hs);
+  for (const void *p : {a->q, a->k, cache ? a->v : nullptr, (const void *)a->q_out,
+                        cache ? nullptr : (const void *)a->k_out, (const void *)a->k_pool,
+                        (const void *)(cache ? a->v_pool : nullptr)})
+    vec = vec && (uintptr_t)p % 16 == 0;
+  if (vec) {
+    uint32_t lg = 0;
+    while ((1u << lg) < lanes)
+      ++lg;
+    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u), groups = kBlock >> lg;
+    const bool many = P.T >= kManyTokens;
+    const uint32_t per = groups * (many ? 4u : 1u);
+    grid.z = (rows + per - 1u) / per;
+    auto fn = a->dtype == SCHED_PD_F32    ? vec_kernel<SCHED_PD_F32>(P.inter, many)
+              : a->dtype == SCHED_PD_BF16 ? vec_kernel<SCHED_PD_BF16>(P.inter, many)
+                                          : vec_kernel<SCHED_PD_F16>(P.inter, many);
+    hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, lg);
+  } else {
+    auto fn = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
+              : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
+                                          : rotary_rows<SCHED_PD_F16>;
+    hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P);
+  }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess)
     return set_error(-1, "sched_qk_norm_rope: launch failed: %s", hipGetErrorString(e));
