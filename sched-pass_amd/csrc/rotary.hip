@@ -254,131 +254,150 @@ template <int N> __device__ __forceinline__ void load_f32(const float *p, float 
   }
 }
 
+// How the vector kernel deals out rows: `lg` = log2 of a row's lanes; ts tokens' rows side
+// by side fill the lane groups of gridDim.z workgroups; a lane group takes `per` such tokens
+// of its row.
+struct Deal {
+  uint32_t lg, ts, per;
+};
+
 // Rows that 16-byte loads reach: L = d / V lanes hold a row (V elements each, L a power
-// of two), so a wave holds 64 / L rows and no lane is idle; the sum of squares and the
-// exchange of the pairs' halves stay within a row's lanes. A workgroup takes U * (256 / L)
-// rows of one token, all their loads in flight together; a lane's angles and weights
-// are those of its dims, loaded once for all of them.
+// of two), so a wave holds 64 / L rows; the sum of squares and the exchange of the
+// pairs' halves stay within a row's lanes. A lane group keeps its row (its weights are
+// loaded once) and walks over tokens, U of them at a time, the next ones' rows and
+// positions on their way while these are turned.
 template <int DT, bool INTER, int U>
-__global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, uint32_t lg) {
+__global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
   constexpr int V = DT == SCHED_PD_F32 ? 4 : 8; // elements of a lane
-  const uint32_t tid = threadIdx.x, L = 1u << lg, li = tid & (L - 1u), grp = tid >> lg;
-  const uint32_t groups = kBlock >> lg, d0 = li * V, half = P.rot / 2u;
+  constexpr int EB = DT == SCHED_PD_F32 ? 4 : 2;
+  constexpr int NC = INTER ? V / 2 : V;         // angles of a lane
+  const uint32_t tid = threadIdx.x, L = 1u << D.lg, li = tid & (L - 1u);
+  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), half = P.rot / 2u, d0 = li * V;
+  const uint32_t f = blockIdx.z * (kBlock >> D.lg) + (tid >> D.lg);
+  const uint32_t tsub = f / rows, row = f - tsub * rows;
   const Span S = span_of(P, blockIdx.x);
-  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), row0 = blockIdx.z * groups * U + grp;
-  const bool turned = d0 < P.rot, first = INTER || d0 < half;
+  const int64_t step = (int64_t)D.ts * D.per;
+  if ((int64_t)blockIdx.y * step >= S.n)
+    return;
+  const bool live = tsub < D.ts;
+  const bool isq = row < P.Hq, isv = row >= P.Hq + P.Hkv;
+  const uint32_t h = isq ? row : isv ? row - P.Hq - P.Hkv : row - P.Hq;
+  const char *src = static_cast<const char *>(isq ? P.q : isv ? P.v : P.k) +
+                    ((int64_t)h * (isq ? P.q_hs : isv ? P.v_hs : P.k_hs) + d0) * EB;
+  const int64_t src_ts = (isq ? P.q_ts : isv ? P.v_ts : P.k_ts) * EB;
+  const bool paged = !isq && P.kp != nullptr;
+  char *dst = static_cast<char *>(isq ? P.qo : !paged ? P.ko : isv ? P.vp : P.kp) +
+              ((int64_t)h * (isq ? P.qo_hs : !paged ? P.ko_hs : isv ? P.vhs : P.khs) + d0) * EB;
+  const int64_t dst_ts = (isq ? P.qo_ts : !paged ? P.ko_ts : isv ? P.vts : P.kts) * EB;
+  const int64_t dst_ps = (isv ? P.vps : P.kps) * EB;
+  const bool turned = !isv && d0 < P.rot, first = INTER || d0 < half;
   // the lane that holds the other halves of this lane's pairs
   const uint32_t hl = half / V;
   const int mate = INTER || !turned ? (int)tid : (int)(first ? tid + hl : tid - hl);
-  const bool has_q = P.qw != nullptr, has_k = P.kw != nullptr;
-  float wq[V], wk[V];
+  const void *w = isv ? nullptr : isq ? P.qw : P.kw;
+  const uint32_t c0 = INTER ? d0 / 2 : first ? d0 : d0 - half;
+  float wt[V];
 #pragma unroll
   for (int e = 0; e < V; ++e)
-    wq[e] = wk[e] = 1.f;
-  if (blockIdx.y < S.n) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) {
-      if (has_q)
-        wq[e] = load_w(P, P.qw, d0 + e);
-      if (has_k)
-        wk[e] = load_w(P, P.kw, d0 + e);
-    }
-  }
-  for (int64_t i = blockIdx.y; i < S.n; i += gridDim.y) {
-    const int64_t tok = S.a0 + i;
-    const int64_t pos = position_of(P, tok);
-    u32x4_t raw[U];
-    const char *src[U];
-    char *dst[U];
-    Place at{-1, 0};
-    if (P.kp)
-      at = place_of(P, S, i);
-    const bool bad = pos < 0 || pos >= (int64_t)P.max_pos;
-    if (blockIdx.z == 0 && tid == 0 && P.errors) {
-      if (bad)
-        atomicAdd(P.errors, 1u);
-      else if (P.kp && at.page < 0)
-        atomicAdd(P.errors, P.Hkv);
-    }
-    if (bad)
-      continue;
-    constexpr int EB = DT == SCHED_PD_F32 ? 4 : 2;
+    wt[e] = w != nullptr && live ? load_w(P, w, d0 + e) : 1.f;
+
+  // token k of this group's walk, the rows outside it as a repeat that is not stored
+  u32x4_t raw[U], nraw[U];
+  int64_t pos[U], npos[U];
+  auto token = [&](int64_t base, uint32_t k) __attribute__((always_inline)) {
+    return base + (int64_t)k * D.ts + tsub;
+  };
+  auto fetch = [&](int64_t base, uint32_t k0) __attribute__((always_inline)) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t row = row0 + u * groups;
-      const bool isq = row < P.Hq, isk = !isq && row < P.Hq + P.Hkv;
-      const uint32_t h = isq ? row : isk ? row - P.Hq : row - P.Hq - P.Hkv;
-      const char *base = static_cast<const char *>(isq ? P.q : isk ? P.k : P.v);
-      const int64_t off = isq   ? tok * P.q_ts + h * P.q_hs
-                          : isk ? tok * P.k_ts + h * P.k_hs
-                                : tok * P.v_ts + h * P.v_hs;
-      src[u] = row < rows ? base + (off + d0) * EB : nullptr;
-      char *to = nullptr;
-      if (isq)
-        to = static_cast<char *>(P.qo) + (tok * P.qo_ts + h * P.qo_hs + d0) * EB;
-      else if (P.kp == nullptr)
-        to = static_cast<char *>(P.ko) + (tok * P.ko_ts + h * P.ko_hs + d0) * EB;
-      else if (at.page >= 0)
-        to = isk ? static_cast<char *>(P.kp) +
-                       (at.page * P.kps + h * P.khs + at.slot * P.kts + d0) * EB
-                 : static_cast<char *>(P.vp) +
-                       (at.page * P.vps + h * P.vhs + at.slot * P.vts + d0) * EB;
-      dst[u] = row < rows ? to : nullptr;
+      const int64_t i = token(base, k0 + u);
+      const bool in = live && k0 + u < D.per && i < S.n;
+      npos[u] = -1;
+      if (in) {
+        npos[u] = position_of(P, S.a0 + i);
+        nraw[u] = *reinterpret_cast<const u32x4_t *>(src + (S.a0 + i) * src_ts);
+      }
     }
+  };
+  for (int64_t base = (int64_t)blockIdx.y * step; base < S.n; base += (int64_t)gridDim.y * step) {
+    fetch(base, 0);
+    for (uint32_t k0 = 0; k0 < D.per; k0 += U) {
+      float c[U][NC], sn[U][NC];
+      char *to[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (src[u] != nullptr)
-        raw[u] = *reinterpret_cast<const u32x4_t *>(src[u]);
-    constexpr int NC = INTER ? V / 2 : V;
-    float c[NC], sn[NC];
-    if (turned) {
-      const float *cs = P.cs + pos * P.cs_stride + (INTER ? d0 / 2 : first ? d0 : d0 - half);
-      load_f32<NC>(cs, c);
-      load_f32<NC>(cs + half, sn);
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const uint32_t row = row0 + u * groups;
-      const bool isq = row < P.Hq, isv = row >= P.Hq + P.Hkv;
-      float x[V];
-      unpack<DT, V>(raw[u], x);
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        ss += x[e] * x[e];
-      for (uint32_t o = L / 2u; o > 0u; o >>= 1)
-        ss += __shfl_xor(ss, (int)o);
-      const bool norm = isq ? has_q : has_k;
-      const float inv = norm ? rsqrtf(ss / (float)P.d + P.eps) : 1.f;
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        x[e] *= inv * (isq ? wq[e] : wk[e]);
-      float y[V];
-      if constexpr (INTER) {
-#pragma unroll
-        for (int e = 0; e < V; e += 2) {
-          y[e] = x[e] * c[e / 2] - x[e + 1] * sn[e / 2];
-          y[e + 1] = x[e + 1] * c[e / 2] + x[e] * sn[e / 2];
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float b = __shfl(x[e], mate);
-          y[e] = first ? x[e] * c[e] - b * sn[e] : x[e] * c[e] + b * sn[e];
+      for (int u = 0; u < U; ++u) {
+        raw[u] = nraw[u], pos[u] = npos[u];
+        const int64_t i = token(base, k0 + u);
+        const bool in = live && k0 + u < D.per && i < S.n;
+        const bool ok = in && pos[u] >= 0 && pos[u] < (int64_t)P.max_pos;
+        to[u] = nullptr;
+        if (ok) {
+          if (paged) {
+            const Place at = place_of(P, S, i);
+            if (at.page >= 0)
+              to[u] = dst + at.page * dst_ps + at.slot * dst_ts;
+            else if (P.errors && row == P.Hq && li == 0u)
+              atomicAdd(P.errors, P.Hkv);
+          } else {
+            to[u] = dst + (S.a0 + i) * dst_ts;
+          }
+          if (turned) {
+            const float *cs = P.cs + pos[u] * P.cs_stride + c0;
+            load_f32<NC>(cs, c[u]);
+            load_f32<NC>(cs + half, sn[u]);
+          }
+        } else if (in && P.errors && row == 0u && li == 0u) {
+          atomicAdd(P.errors, 1u);
         }
       }
+      if (k0 + U < D.per)
+        fetch(base, k0 + U);
 #pragma unroll
-      for (int e = 0; e < V; ++e)
-        y[e] = turned ? y[e] : x[e];
-      if (dst[u] != nullptr)
-        *reinterpret_cast<u32x4_t *>(dst[u]) = isv ? raw[u] : pack<DT, V>(y);
+      for (int u = 0; u < U; ++u) {
+        float x[V], y[V];
+        unpack<DT, V>(raw[u], x);
+        float ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          ss += x[e] * x[e];
+        for (uint32_t o = L / 2u; o > 0u; o >>= 1)
+          ss += __shfl_xor(ss, (int)o);
+        const float inv = w != nullptr ? rsqrtf(ss / (float)P.d + P.eps) : 1.f;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          x[e] *= inv * wt[e];
+        if constexpr (INTER) {
+#pragma unroll
+          for (int e = 0; e < V; e += 2) {
+            y[e] = x[e] * c[u][e / 2] - x[e + 1] * sn[u][e / 2];
+            y[e + 1] = x[e + 1] * c[u][e / 2] + x[e] * sn[u][e / 2];
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const float b = __shfl(x[e], mate);
+            y[e] = first ? x[e] * c[u][e] - b * sn[u][e] : x[e] * c[u][e] + b * sn[u][e];
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          y[e] = turned ? y[e] : x[e];
+        if (to[u] != nullptr)
+          *reinterpret_cast<u32x4_t *>(to[u]) = isv ? raw[u] : pack<DT, V>(y);
+      }
     }
   }
 }
 
+#ifndef NU
+#define NU 2
+#endif
+#ifndef NPER
+#define NPER 8
+#endif
 template <int DT> auto vec_kernel(bool inter, bool many) {
-  return inter ? (many ? rotary_vec<DT, true, 4> : rotary_vec<DT, true, 1>)
-               : (many ? rotary_vec<DT, false, 4> : rotary_vec<DT, false, 1>);
+  return inter ? (many ? rotary_vec<DT, true, NU> : rotary_vec<DT, true, 1>)
+               : (many ? rotary_vec<DT, false, NU> : rotary_vec<DT, false, 1>);
 }
 
 uint32_t esize(uint32_t dt) { return dt == SCHED_PD_F32 ? 4u : 2u; }
@@ -497,17 +516,28 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
                         (const void *)(cache ? a->v_pool : nullptr)})
     vec = vec && (uintptr_t)p % 16 == 0;
   if (vec) {
-    uint32_t lg = 0;
-    while ((1u << lg) < lanes)
-      ++lg;
-    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u), groups = kBlock >> lg;
+    Deal D{};
+    while ((1u << D.lg) < lanes)
+      ++D.lg;
+    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u), groups = kBlock >> D.lg;
     const bool many = P.T >= kManyTokens;
-    const uint32_t per = groups * (many ? 4u : 1u);
-    grid.z = (rows + per - 1u) / per;
+    // as many tokens side by side as leave few lane groups idle, at most 8
+    D.ts = 1;
+    if (many)
+      for (uint32_t t = 1, best = ~0u; t <= 8; ++t) {
+        const uint32_t z = (t * rows + groups - 1u) / groups;
+        const uint32_t idle = (z * groups - t * rows) * 1000u / (z * groups);
+        if (idle < best)
+          best = idle, D.ts = t;
+      }
+    D.per = many ? NPER : 1u;
+    grid.z = (D.ts * rows + groups - 1u) / groups;
+    const uint64_t gy = ((uint64_t)most + D.ts * D.per - 1u) / (D.ts * D.per);
+    grid.y = (uint32_t)(gy < 65535u ? gy : 65535u);
     auto fn = a->dtype == SCHED_PD_F32    ? vec_kernel<SCHED_PD_F32>(P.inter, many)
               : a->dtype == SCHED_PD_BF16 ? vec_kernel<SCHED_PD_BF16>(P.inter, many)
                                           : vec_kernel<SCHED_PD_F16>(P.inter, many);
-    hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, lg);
+    hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, D);
   } else {
     auto fn = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
               : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
