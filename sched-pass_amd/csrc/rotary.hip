@@ -22,10 +22,13 @@ namespace {
 
 constexpr int kBlock = 256;
 #ifndef MANYT
-#define MANYT 1024
+#define MANYT 2048
 #endif
-// From this many tokens on a workgroup takes four rounds of a token's rows, below one.
-constexpr uint32_t kManyTokens = MANYT;
+#ifndef NPER
+#define NPER 8
+#endif
+// From this many tokens on a lane group takes several of them, below one.
+constexpr uint32_t kManyTokens = MANYT, kTokensPer = NPER;
 
 struct RParams {
   const void *q, *k, *v;
@@ -66,10 +69,18 @@ template <int DT> __device__ __forceinline__ void st(void *p, int64_t i, float v
     static_cast<_Float16 *>(p)[i] = (_Float16)v;
 }
 
+// 16 bits as a bf16 or an fp16, by a select: as one of three branches per element, under a
+// lane's condition, hipcc 7.2 left a register of the fp16 branch unset (the row's
+// address was built from it).
+__device__ __forceinline__ float half_w(uint32_t w_dtype, uint32_t b) {
+  const float x = bf16_bits_to_f32(b), y = (float)__builtin_bit_cast(_Float16, (uint16_t)b);
+  return w_dtype == SCHED_PD_BF16 ? x : y;
+}
+
 __device__ __forceinline__ float load_w(const RParams &P, const void *w, uint32_t j) {
-  return P.w_dtype == SCHED_PD_F32    ? ld<SCHED_PD_F32>(w, j)
-         : P.w_dtype == SCHED_PD_BF16 ? ld<SCHED_PD_BF16>(w, j)
-                                      : ld<SCHED_PD_F16>(w, j);
+  if (P.w_dtype == SCHED_PD_F32)
+    return static_cast<const float *>(w)[j];
+  return half_w(P.w_dtype, static_cast<const uint16_t *>(w)[j]);
 }
 
 __device__ __forceinline__ float wave_sum(float x) {
@@ -254,26 +265,68 @@ template <int N> __device__ __forceinline__ void load_f32(const float *p, float 
   }
 }
 
-// How the vector kernel deals out rows: `lg` = log2 of a row's lanes; ts tokens' rows side
-// by side fill the lane groups of gridDim.z workgroups; a lane group takes `per` such tokens
-// of its row.
+// x of the lane that differs in bit HLG of its number, by VALU moves: quad permutes, row
+// shifts with the banks that take them, a row rotation, the row swaps.
+template <int HLG> __device__ __forceinline__ float xor_lane(float x) {
+  const int i = __float_as_int(x);
+  if constexpr (HLG == 0)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0xB1, 0xF, 0xF, false));
+  else if constexpr (HLG == 1)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x4E, 0xF, 0xF, false));
+  else if constexpr (HLG == 2) { // banks 0, 2 from 4 lanes up, banks 1, 3 from 4 down
+    const int a = __builtin_amdgcn_update_dpp(0, i, 0x104, 0xF, 0x5, false);
+    return __int_as_float(__builtin_amdgcn_update_dpp(a, i, 0x114, 0xF, 0xA, false));
+  } else if constexpr (HLG == 3)
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, i, 0x128, 0xF, 0xF, false));
+  else if constexpr (HLG == 4) {
+    const auto a = __builtin_amdgcn_permlane16_swap((unsigned)i, (unsigned)i, false, false);
+    return __uint_as_float((threadIdx.x & 16u) ? a[0] : a[1]);
+  } else {
+    const auto a = __builtin_amdgcn_permlane32_swap((unsigned)i, (unsigned)i, false, false);
+    return __uint_as_float((threadIdx.x & 32u) ? a[0] : a[1]);
+  }
+}
+
+// The sum over the 2^LG lanes of a row, on every one of them.
+template <int LG> __device__ __forceinline__ float row_sum(float x) {
+  if constexpr (LG > 0)
+    x += xor_lane<0>(x);
+  if constexpr (LG > 1)
+    x += xor_lane<1>(x);
+  if constexpr (LG > 2)
+    x += xor_lane<2>(x);
+  if constexpr (LG > 3)
+    x += xor_lane<3>(x);
+  if constexpr (LG > 4)
+    x += xor_lane<4>(x);
+  if constexpr (LG > 5)
+    x += xor_lane<5>(x);
+  return x;
+}
+
+// How the vector kernel deals out rows: ts tokens' rows side by side fill the lane groups of
+// gridDim.z workgroups; a lane group takes `per` such tokens of its row.
 struct Deal {
-  uint32_t lg, ts, per;
+  uint32_t ts, per;
+  float inv_d;
 };
 
-// Rows that 16-byte loads reach: L = d / V lanes hold a row (V elements each, L a power
-// of two), so a wave holds 64 / L rows; the sum of squares and the exchange of the
-// pairs' halves stay within a row's lanes. A lane group keeps its row (its weights are
-// loaded once) and walks over tokens, U of them at a time, the next ones' rows and
-// positions on their way while these are turned.
-template <int DT, bool INTER, int U>
+// Rows that 16-byte loads reach: 2^LG lanes hold a row (V elements each), so a wave holds
+// 64 >> LG rows; the sum of squares and the exchange of the pairs' halves (HLG: lanes whose
+// numbers differ in that bit hold them; -1: neighbouring pairs, within a lane) stay within
+// a row's lanes, in VALU moves. A lane group keeps its row (its weights are loaded once)
+// and walks over tokens, U of them at a time, the next ones' rows and positions on their
+// way while these are turned.
+template <int DT, int LG, int HLG, int U>
 __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
+  constexpr bool INTER = HLG < 0;
   constexpr int V = DT == SCHED_PD_F32 ? 4 : 8; // elements of a lane
   constexpr int EB = DT == SCHED_PD_F32 ? 4 : 2;
   constexpr int NC = INTER ? V / 2 : V;         // angles of a lane
-  const uint32_t tid = threadIdx.x, L = 1u << D.lg, li = tid & (L - 1u);
+  constexpr uint32_t L = 1u << LG;
+  const uint32_t tid = threadIdx.x, li = tid & (L - 1u);
   const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), half = P.rot / 2u, d0 = li * V;
-  const uint32_t f = blockIdx.z * (kBlock >> D.lg) + (tid >> D.lg);
+  const uint32_t f = blockIdx.z * (kBlock >> LG) + (tid >> LG);
   const uint32_t tsub = f / rows, row = f - tsub * rows;
   const Span S = span_of(P, blockIdx.x);
   const int64_t step = (int64_t)D.ts * D.per;
@@ -282,56 +335,67 @@ __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
   const bool live = tsub < D.ts;
   const bool isq = row < P.Hq, isv = row >= P.Hq + P.Hkv;
   const uint32_t h = isq ? row : isv ? row - P.Hq - P.Hkv : row - P.Hq;
+  const bool paged = !isq && P.kp != nullptr;
+  const bool turned = !isv && d0 < P.rot, first = INTER || d0 < half;
+  const void *w = isv ? nullptr : isq ? P.qw : P.kw;
+  float wt[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e)
+    wt[e] = 1.f;
+  if (w != nullptr && live) {
+    if (P.w_dtype == SCHED_PD_F32) {
+      load_f32<V>(static_cast<const float *>(w) + d0, wt);
+    } else {
+      const uint2 *p = reinterpret_cast<const uint2 *>(static_cast<const uint16_t *>(w) + d0);
+#pragma unroll
+      for (int k = 0; k < V / 4; ++k) {
+        const uint2 b = p[k];
+        wt[4 * k] = half_w(P.w_dtype, b.x & 0xffffu);
+        wt[4 * k + 1] = half_w(P.w_dtype, b.x >> 16);
+        wt[4 * k + 2] = half_w(P.w_dtype, b.y & 0xffffu);
+        wt[4 * k + 3] = half_w(P.w_dtype, b.y >> 16);
+      }
+    }
+  }
   const char *src = static_cast<const char *>(isq ? P.q : isv ? P.v : P.k) +
                     ((int64_t)h * (isq ? P.q_hs : isv ? P.v_hs : P.k_hs) + d0) * EB;
   const int64_t src_ts = (isq ? P.q_ts : isv ? P.v_ts : P.k_ts) * EB;
-  const bool paged = !isq && P.kp != nullptr;
   char *dst = static_cast<char *>(isq ? P.qo : !paged ? P.ko : isv ? P.vp : P.kp) +
               ((int64_t)h * (isq ? P.qo_hs : !paged ? P.ko_hs : isv ? P.vhs : P.khs) + d0) * EB;
   const int64_t dst_ts = (isq ? P.qo_ts : !paged ? P.ko_ts : isv ? P.vts : P.kts) * EB;
   const int64_t dst_ps = (isv ? P.vps : P.kps) * EB;
-  const bool turned = !isv && d0 < P.rot, first = INTER || d0 < half;
-  // the lane that holds the other halves of this lane's pairs
-  const uint32_t hl = half / V;
-  const int mate = INTER || !turned ? (int)tid : (int)(first ? tid + hl : tid - hl);
-  const void *w = isv ? nullptr : isq ? P.qw : P.kw;
-  const uint32_t c0 = INTER ? d0 / 2 : first ? d0 : d0 - half;
-  float wt[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e)
-    wt[e] = w != nullptr && live ? load_w(P, w, d0 + e) : 1.f;
+  const float *cs0 = P.cs + (INTER ? d0 / 2 : first ? d0 : d0 - half);
 
-  // token k of this group's walk, the rows outside it as a repeat that is not stored
-  u32x4_t raw[U], nraw[U];
-  int64_t pos[U], npos[U];
-  auto token = [&](int64_t base, uint32_t k) __attribute__((always_inline)) {
-    return base + (int64_t)k * D.ts + tsub;
-  };
-  auto fetch = [&](int64_t base, uint32_t k0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int64_t i = token(base, k0 + u);
-      const bool in = live && k0 + u < D.per && i < S.n;
-      npos[u] = -1;
-      if (in) {
-        npos[u] = position_of(P, S.a0 + i);
-        nraw[u] = *reinterpret_cast<const u32x4_t *>(src + (S.a0 + i) * src_ts);
-      }
-    }
-  };
   for (int64_t base = (int64_t)blockIdx.y * step; base < S.n; base += (int64_t)gridDim.y * step) {
-    fetch(base, 0);
+    // this group's tokens base + tsub + k ts, k < cnt
+    const int64_t i0 = base + tsub, end = base + step < S.n ? base + step : S.n;
+    const uint32_t cnt = live && i0 < end ? (uint32_t)((end - i0 + D.ts - 1) / D.ts) : 0u;
+    const char *from = src + (S.a0 + i0) * src_ts;
+    const int64_t hop = (int64_t)D.ts * src_ts;
+    u32x4_t raw[U], nraw[U];
+    int64_t pos[U], npos[U];
+    auto fetch = [&](uint32_t k0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (k0 + u < cnt) {
+          npos[u] = position_of(P, S.a0 + i0 + (int64_t)(k0 + u) * D.ts);
+          nraw[u] = *reinterpret_cast<const u32x4_t *>(from);
+        }
+        from += hop;
+      }
+    };
+    fetch(0);
     for (uint32_t k0 = 0; k0 < D.per; k0 += U) {
       float c[U][NC], sn[U][NC];
       char *to[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
         raw[u] = nraw[u], pos[u] = npos[u];
-        const int64_t i = token(base, k0 + u);
-        const bool in = live && k0 + u < D.per && i < S.n;
-        const bool ok = in && pos[u] >= 0 && pos[u] < (int64_t)P.max_pos;
         to[u] = nullptr;
-        if (ok) {
+        if (k0 + u >= cnt)
+          continue;
+        const int64_t i = i0 + (int64_t)(k0 + u) * D.ts;
+        if ((uint64_t)pos[u] < (uint64_t)P.max_pos) {
           if (paged) {
             const Place at = place_of(P, S, i);
             if (at.page >= 0)
@@ -342,62 +406,101 @@ __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
             to[u] = dst + (S.a0 + i) * dst_ts;
           }
           if (turned) {
-            const float *cs = P.cs + pos[u] * P.cs_stride + c0;
+            const float *cs = cs0 + pos[u] * P.cs_stride;
             load_f32<NC>(cs, c[u]);
             load_f32<NC>(cs + half, sn[u]);
           }
-        } else if (in && P.errors && row == 0u && li == 0u) {
+        } else if (P.errors && row == 0u && li == 0u) {
           atomicAdd(P.errors, 1u);
         }
       }
       if (k0 + U < D.per)
-        fetch(base, k0 + U);
+        fetch(k0 + U);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        float x[V], y[V];
+        float x[V];
         unpack<DT, V>(raw[u], x);
         float ss = 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e)
           ss += x[e] * x[e];
-        for (uint32_t o = L / 2u; o > 0u; o >>= 1)
-          ss += __shfl_xor(ss, (int)o);
-        const float inv = w != nullptr ? rsqrtf(ss / (float)P.d + P.eps) : 1.f;
+        ss = row_sum<LG>(ss);
+        const float inv = w != nullptr ? rsqrtf(ss * D.inv_d + P.eps) : 1.f;
 #pragma unroll
         for (int e = 0; e < V; ++e)
           x[e] *= inv * wt[e];
         if constexpr (INTER) {
+          if (turned) {
 #pragma unroll
-          for (int e = 0; e < V; e += 2) {
-            y[e] = x[e] * c[u][e / 2] - x[e + 1] * sn[u][e / 2];
-            y[e + 1] = x[e + 1] * c[u][e / 2] + x[e] * sn[u][e / 2];
+            for (int e = 0; e < V; e += 2) {
+              const float a = x[e], b = x[e + 1];
+              x[e] = a * c[u][e / 2] - b * sn[u][e / 2];
+              x[e + 1] = b * c[u][e / 2] + a * sn[u][e / 2];
+            }
           }
         } else {
+          float b[V];
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float b = __shfl(x[e], mate);
-            y[e] = first ? x[e] * c[u][e] - b * sn[u][e] : x[e] * c[u][e] + b * sn[u][e];
+          for (int e = 0; e < V; ++e)
+            b[e] = xor_lane<HLG>(x[e]); // every lane takes part
+          if (turned) {
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+              x[e] = x[e] * c[u][e] + (first ? -b[e] : b[e]) * sn[u][e];
           }
         }
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          y[e] = turned ? y[e] : x[e];
         if (to[u] != nullptr)
-          *reinterpret_cast<u32x4_t *>(to[u]) = isv ? raw[u] : pack<DT, V>(y);
+          *reinterpret_cast<u32x4_t *>(to[u]) = isv ? raw[u] : pack<DT, V>(x);
       }
     }
   }
 }
 
-#ifndef NU
-#define NU 2
-#endif
-#ifndef NPER
-#define NPER 8
-#endif
-template <int DT> auto vec_kernel(bool inter, bool many) {
-  return inter ? (many ? rotary_vec<DT, true, NU> : rotary_vec<DT, true, 1>)
-               : (many ? rotary_vec<DT, false, NU> : rotary_vec<DT, false, 1>);
+typedef void (*VecFn)(RParams, Deal);
+
+// A row's lanes (log2) and the lane bit that pairs' halves differ in (-1: none): full,
+// half and quarter rotation of a head.
+template <int DT, int LG, int U> VecFn vec_of(int hlg) {
+  if (hlg < 0)
+    return rotary_vec<DT, LG, -1, U>;
+  if (hlg == LG - 1)
+    return rotary_vec<DT, LG, LG - 1, U>;
+  if (hlg == LG - 2)
+    return rotary_vec<DT, LG, LG - 2, U>;
+  if constexpr (LG >= 3)
+    if (hlg == LG - 3)
+      return rotary_vec<DT, LG, LG - 3, U>;
+  return nullptr;
+}
+
+template <int DT, int U> VecFn vec_of(int lg, int hlg) {
+  if (lg == 2)
+    return vec_of<DT, 2, U>(hlg);
+  if (lg == 3)
+    return vec_of<DT, 3, U>(hlg);
+  if (lg == 4)
+    return vec_of<DT, 4, U>(hlg);
+  if (lg == 5)
+    return vec_of<DT, 5, U>(hlg);
+  if constexpr (DT == SCHED_PD_F32)
+    if (lg == 6)
+      return vec_of<DT, 6, U>(hlg);
+  return nullptr;
+}
+
+template <int U> VecFn vec_of(uint32_t dt, int lg, int hlg) {
+  return dt == SCHED_PD_F32    ? vec_of<SCHED_PD_F32, U>(lg, hlg)
+         : dt == SCHED_PD_BF16 ? vec_of<SCHED_PD_BF16, U>(lg, hlg)
+                               : vec_of<SCHED_PD_F16, U>(lg, hlg);
+}
+
+int log2_of(uint32_t x) { // -1: not a power of two
+  if (x == 0 || (x & (x - 1u)))
+    return -1;
+  int n = 0;
+  while ((1u << n) < x)
+    ++n;
+  return n;
 }
 
 uint32_t esize(uint32_t dt) { return dt == SCHED_PD_F32 ? 4u : 2u; }
@@ -499,13 +602,12 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
   dim3 grid(cache ? a->num_requests : 1u, most < 65535u ? most : 65535u);
   hipStream_t s = static_cast<hipStream_t>(stream);
   // 16-byte pieces: whole in each row, aligned everywhere, pairs' halves in whole pieces
-  const uint32_t v = 16u / es, lanes = a->head_dim / v;
+  const uint32_t v = 16u / es;
   auto pieces = [&](int64_t x) { return x % v == 0; };
-  bool vec = a->head_dim % v == 0 && lanes >= 1 && lanes <= 64 && (lanes & (lanes - 1u)) == 0 &&
-             pieces(P.q_ts) && pieces(P.q_hs) && pieces(P.k_ts) && pieces(P.k_hs) &&
-             pieces(P.qo_ts) && pieces(P.qo_hs) && a->rot_dim % v == 0 &&
-             (P.inter || (a->rot_dim / 2u) % v == 0) && a->cs_stride % 4 == 0 &&
-             (uintptr_t)a->cos_sin % 16 == 0 && (a->rot_dim / 2u) % 4 == 0;
+  bool vec = a->head_dim % v == 0 && a->rot_dim % v == 0 && a->cs_stride % 4 == 0 &&
+             (P.inter || (a->rot_dim / 2u) % v == 0) && (a->rot_dim / 2u) % 4 == 0 &&
+             (uintptr_t)a->cos_sin % 16 == 0 && pieces(P.q_ts) && pieces(P.q_hs) &&
+             pieces(P.k_ts) && pieces(P.k_hs) && pieces(P.qo_ts) && pieces(P.qo_hs);
   if (cache)
     vec = vec && pieces(P.v_ts) && pieces(P.v_hs) && pieces(P.kps) && pieces(P.khs) &&
           pieces(P.kts) && pieces(P.vps) && pieces(P.vhs) && pieces(P.vts);
@@ -515,34 +617,35 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
                         cache ? nullptr : (const void *)a->k_out, (const void *)a->k_pool,
                         (const void *)(cache ? a->v_pool : nullptr)})
     vec = vec && (uintptr_t)p % 16 == 0;
+  for (const void *p : {a->q_weight, a->k_weight})
+    vec = vec && (uintptr_t)p % (a->w_dtype == SCHED_PD_F32 ? 16 : 8) == 0;
+  VecFn fn = nullptr;
+  const bool many = P.T >= kManyTokens;
   if (vec) {
-    Deal D{};
-    while ((1u << D.lg) < lanes)
-      ++D.lg;
-    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u), groups = kBlock >> D.lg;
-    const bool many = P.T >= kManyTokens;
-    // as many tokens side by side as leave few lane groups idle, at most 8
-    D.ts = 1;
-    if (many)
+    const int lg = log2_of(a->head_dim / v), hlg = P.inter ? -1 : log2_of(a->rot_dim / 2u / v);
+    if (lg >= 0 && (P.inter || hlg >= 0))
+      fn = many ? vec_of<2>(a->dtype, lg, hlg) : vec_of<1>(a->dtype, lg, hlg);
+  }
+  if (fn) {
+    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u);
+    const uint32_t groups = kBlock / (a->head_dim / v);
+    Deal D{1u, many ? kTokensPer : 1u, 1.f / (float)a->head_dim};
+    if (many) // as many tokens side by side, at most 8, as leave the fewest lane groups idle
       for (uint32_t t = 1, best = ~0u; t <= 8; ++t) {
         const uint32_t z = (t * rows + groups - 1u) / groups;
         const uint32_t idle = (z * groups - t * rows) * 1000u / (z * groups);
         if (idle < best)
           best = idle, D.ts = t;
       }
-    D.per = many ? NPER : 1u;
     grid.z = (D.ts * rows + groups - 1u) / groups;
     const uint64_t gy = ((uint64_t)most + D.ts * D.per - 1u) / (D.ts * D.per);
     grid.y = (uint32_t)(gy < 65535u ? gy : 65535u);
-    auto fn = a->dtype == SCHED_PD_F32    ? vec_kernel<SCHED_PD_F32>(P.inter, many)
-              : a->dtype == SCHED_PD_BF16 ? vec_kernel<SCHED_PD_BF16>(P.inter, many)
-                                          : vec_kernel<SCHED_PD_F16>(P.inter, many);
     hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, D);
   } else {
-    auto fn = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
-              : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
-                                          : rotary_rows<SCHED_PD_F16>;
-    hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P);
+    auto every = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
+                 : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
+                                             : rotary_rows<SCHED_PD_F16>;
+    hipLaunchKernelGGL(every, grid, dim3(kBlock), 0, s, P);
   }
   hipError_t e = hipGetLastError();
   if (e != hipSuccess)
