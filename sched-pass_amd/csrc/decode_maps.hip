@@ -198,10 +198,13 @@ __device__ __forceinline__ void join_rows(const MapParams &P, uint64_t item0, ui
 }
 
 // The join of what `maps_valu` and, for tasks of several chunks, maps_mfma left:
-// workgroup (task, y). y < G: q-head y's output; from there on the weights, their tokens dealt
-// out over the workgroups. A dim's chunks are summed by kJoin / D lanes, 8 loads in flight
-// each, and their sums in order.
-template <int D, bool DIFF> __global__ void __launch_bounds__(kJoin) maps_join(MapParams P) {
+// workgroup (task, y). y < outs: the outputs of q-heads y, y + outs, ...; from there on the
+// weights, kTokens tokens a workgroup and round. A dim's chunks are summed by kJoin / D lanes,
+// 8 loads in flight each, and their sums in order.
+constexpr uint32_t kTokens = 4 * kJoin;
+
+template <int D, bool DIFF>
+__global__ void __launch_bounds__(kJoin) maps_join(MapParams P, uint32_t outs) {
   constexpr uint32_t LANES = kJoin / D, NR = DIFF ? 2 : 1, CH = 64;
   __shared__ float s_M[kMostRows], s_Li[kMostRows];
   __shared__ float s_f[NR][CH], s_o[NR][LANES][D], s_sum[kJoin / 64];
@@ -212,82 +215,88 @@ template <int D, bool DIFF> __global__ void __launch_bounds__(kJoin) maps_join(M
   if (nch <= P.join_from)
     return; // the stream has finished this task
   const uint64_t item0 = (uint64_t)task * P.nsplit;
-  if (blockIdx.y < P.G) {
-    const uint32_t g = blockIdx.y, g0 = g * NR, hq = h * P.G + g;
-    join_rows(P, item0, nch, g0, g0 + NR, s_M, s_Li);
+  if (blockIdx.y < outs) {
+    if (outs == 1u)
+      join_rows(P, item0, nch, 0u, P.rows, s_M, s_Li);
+    else
+      join_rows(P, item0, nch, blockIdx.y * NR, blockIdx.y * NR + NR, s_M, s_Li);
     const uint32_t j = tid % D, part = tid / D;
-    float o[NR] = {};
-    for (uint32_t c0 = 0; c0 < nch; c0 += CH) {
-      const uint32_t cnt = min(CH, nch - c0);
-      __syncthreads(); // the rows are joined; the previous shares have been used
-      if (tid < NR * CH) {
-        const uint32_t k = tid / CH, c = tid % CH;
-        s_f[k][c] = c < cnt ? __builtin_amdgcn_exp2f(P.ml[((item0 + c0 + c) * P.rows + g0 + k) * 2u] -
-                                                     s_M[g0 + k]) * s_Li[g0 + k]
-                            : 0.f;
-      }
-      __syncthreads();
-      for (uint32_t c = part; c < cnt; c += 8u * LANES) {
-        float v[8][NR];
-#pragma unroll
-        for (uint32_t u = 0; u < 8; ++u) {
-          const uint32_t cc = min(c + u * LANES, cnt - 1u);
-#pragma unroll
-          for (uint32_t k = 0; k < NR; ++k)
-            v[u][k] = P.acc[((item0 + c0 + cc) * P.rows + g0 + k) * D + j];
+    for (uint32_t g = blockIdx.y; g < P.G; g += outs) {
+      const uint32_t g0 = g * NR, hq = h * P.G + g;
+      float o[NR] = {};
+      for (uint32_t c0 = 0; c0 < nch; c0 += CH) {
+        const uint32_t cnt = min(CH, nch - c0);
+        __syncthreads(); // the rows are joined; the previous shares have been used
+        if (tid < NR * CH) {
+          const uint32_t k = tid / CH, c = tid % CH;
+          s_f[k][c] = c < cnt ? __builtin_amdgcn_exp2f(
+                                    P.ml[((item0 + c0 + c) * P.rows + g0 + k) * 2u] - s_M[g0 + k]) *
+                                    s_Li[g0 + k]
+                              : 0.f;
         }
-#pragma unroll
-        for (uint32_t u = 0; u < 8; ++u)
-#pragma unroll
-          for (uint32_t k = 0; k < NR; ++k)
-            if (c + u * LANES < cnt)
-              o[k] += v[u][k] * s_f[k][c + u * LANES];
-      }
-    }
-#pragma unroll
-    for (uint32_t k = 0; k < NR; ++k)
-      s_o[k][part][j] = o[k];
-    __syncthreads();
-    float x = 0.f;
-    if (tid < D) {
-      float t[NR];
-#pragma unroll
-      for (uint32_t k = 0; k < NR; ++k) {
-        t[k] = s_o[k][0][tid];
-#pragma unroll
-        for (uint32_t q = 1; q < LANES; ++q)
-          t[k] += s_o[k][q][tid];
-      }
-      x = t[0];
-      if constexpr (DIFF)
-        x -= P.lam[hq] * t[NR - 1];
-    }
-    if constexpr (DIFF) {
-      float inv = P.mul;
-      if (P.nw) {
-        float ss = x * x;
-#pragma unroll
-        for (int k = 32; k > 0; k >>= 1)
-          ss += __shfl_xor(ss, k);
-        if ((tid & 63u) == 0u)
-          s_sum[tid >> 6] = ss;
         __syncthreads();
-        ss = s_sum[0];
+        for (uint32_t c = part; c < cnt; c += 8u * LANES) {
+          float v[8][NR];
 #pragma unroll
-        for (int k = 1; k < D / 64; ++k)
-          ss += s_sum[k];
-        inv *= rsqrtf(ss / (float)D + P.eps);
-        if (tid < D)
-          inv *= P.nw[tid];
+          for (uint32_t u = 0; u < 8; ++u) {
+            const uint32_t cc = min(c + u * LANES, cnt - 1u);
+#pragma unroll
+            for (uint32_t k = 0; k < NR; ++k)
+              v[u][k] = P.acc[((item0 + c0 + cc) * P.rows + g0 + k) * D + j];
+          }
+#pragma unroll
+          for (uint32_t u = 0; u < 8; ++u)
+#pragma unroll
+            for (uint32_t k = 0; k < NR; ++k)
+              if (c + u * LANES < cnt)
+                o[k] += v[u][k] * s_f[k][c + u * LANES];
+        }
       }
-      x *= inv;
+#pragma unroll
+      for (uint32_t k = 0; k < NR; ++k)
+        s_o[k][part][j] = o[k];
+      __syncthreads();
+      float x = 0.f;
+      if (tid < D) {
+        float t[NR];
+#pragma unroll
+        for (uint32_t k = 0; k < NR; ++k) {
+          t[k] = s_o[k][0][tid];
+#pragma unroll
+          for (uint32_t q = 1; q < LANES; ++q)
+            t[k] += s_o[k][q][tid];
+        }
+        x = t[0];
+        if constexpr (DIFF)
+          x -= P.lam[hq] * t[NR - 1];
+      }
+      if constexpr (DIFF) {
+        float inv = P.mul;
+        if (P.nw) {
+          float ss = x * x;
+#pragma unroll
+          for (int k = 32; k > 0; k >>= 1)
+            ss += __shfl_xor(ss, k);
+          if ((tid & 63u) == 0u)
+            s_sum[tid >> 6] = ss;
+          __syncthreads();
+          ss = s_sum[0];
+#pragma unroll
+          for (int k = 1; k < D / 64; ++k)
+            ss += s_sum[k];
+          inv *= rsqrtf(ss / (float)D + P.eps);
+          if (tid < D)
+            inv *= P.nw[tid];
+        }
+        x *= inv;
+      }
+      if (tid < D)
+        map_store(P, ((int64_t)r * P.Hq + hq) * D + tid, n ? x : __builtin_nanf(""));
     }
-    if (tid < D)
-      map_store(P, ((int64_t)r * P.Hq + hq) * D + tid, n ? x : __builtin_nanf(""));
     return;
   }
   if constexpr (!DIFF) {
-    const uint32_t first = (blockIdx.y - P.G) * kJoin, stride = (gridDim.y - P.G) * kJoin;
+    const uint32_t first = (blockIdx.y - outs) * kTokens, stride = (gridDim.y - outs) * kTokens;
     if (first >= n)
       return;
     join_rows(P, item0, nch, 0u, P.rows, s_M, s_Li);
@@ -295,18 +304,10 @@ template <int D, bool DIFF> __global__ void __launch_bounds__(kJoin) maps_join(M
     const int64_t row = map_row(P, r);
     const int64_t have = P.counted ? (int64_t)P.counted[r] : (int64_t)n;
     __syncthreads();
-    for (uint32_t t = first + tid; t < n; t += stride) {
+    for (uint32_t t = first + tid * 4u; t < n; t += stride) {
       const uint32_t page = (uint32_t)P.bt[row + t / P.ps];
-      if (page >= P.num_pages || b0 + t / 16u >= P.score_blocks)
-        continue;
-      const float *s = score_block(P, b0, t / 16u, h) + (t & 15u);
-      float *w = P.w + (int64_t)page * P.w_ps + (int64_t)h * P.w_hs + t % P.ps;
-      const float old = (int64_t)t < have ? *w * P.decay : 0.f;
-      float a = 0.f;
-#pragma unroll 4
-      for (uint32_t g = 0; g < P.rows; ++g)
-        a += __builtin_amdgcn_exp2f(s[g * 16u] - s_M[g]) * s_Li[g];
-      *w = old + a;
+      if (page < P.num_pages && b0 + t / 16u < P.score_blocks)
+        map_weights4(P, h, page, t, n, have, score_block(P, b0, t / 16u, h) + (t & 15u), s_M, s_Li);
     }
   }
 }
@@ -327,7 +328,7 @@ uint64_t elem_bytes(uint32_t dt) {
 // What a call's shape decides: how far tasks are split, and the workspace.
 struct Plan {
   bool mfma;
-  uint32_t rows, nsplit, least;
+  uint32_t rows, nsplit, chunk;
   uint64_t score_blocks, ml_off, acc_off, total;
 };
 
@@ -397,18 +398,24 @@ bool mfma_applies(const SchedMapsArgs *a) {
          ((uintptr_t)a->q & 15u) == 0;
 }
 
-// Chunks fill the card this many times over; none is shorter than kLeastTokens. A weighted
-// chunk's scores fit kScoreBytes of LDS on the matrix cores.
-#ifndef ITEMS
-#define ITEMS 1024
+// How tasks are cut (map_chunk): into chunks of 8 tokens for each task of the call, between
+// kLeastChunk and kMostChunk, so that a few long tasks fill the card and many tasks stay
+// whole, but for the longest. Longer ones where a wide table would make more than kMostSplit
+// chunks of a task or kMostItems of the call; on the matrix cores a weighted chunk's
+// scores fit kScoreBytes of LDS.
+#ifndef LEASTC
+#define LEASTC 256
 #endif
-#ifndef LEAST
-#define LEAST 256
+#ifndef MOSTC
+#define MOSTC 2048
+#endif
+#ifndef PERT
+#define PERT 8
 #endif
 #ifndef SCB
 #define SCB 40
 #endif
-constexpr uint32_t kItems = ITEMS, kLeastTokens = LEAST, kMostSplit = 64;
+constexpr uint64_t kLeastChunk = LEASTC, kMostChunk = MOSTC, kMostSplit = 128, kMostItems = 4096;
 constexpr uint32_t kScoreBytes = SCB << 10;
 
 Plan plan_of(const SchedMapsArgs *a) {
@@ -418,15 +425,15 @@ Plan plan_of(const SchedMapsArgs *a) {
   const bool weighted = a->op == SCHED_MAPS_WEIGHTED;
   p.mfma = mfma_applies(a);
   p.rows = a->num_q_heads / a->num_kv_heads * (weighted ? 1u : 2u);
-  p.least = kLeastTokens;
-  uint64_t want = (kItems + tasks - 1) / tasks;
-  const uint64_t can = (longest + p.least - 1) / p.least;
-  want = std::min<uint64_t>({want, can, kMostSplit});
-  if (weighted && p.mfma) {
-    const uint64_t fits = kScoreBytes / (p.rows * 4u) / 64u * 64u; // (chunks are 64s of tokens)
-    want = std::max<uint64_t>(want, (longest + fits - 1) / fits);
-  }
-  p.nsplit = (uint32_t)std::max<uint64_t>(1, want);
+  uint64_t chunk = std::min(std::max(PERT * tasks, kLeastChunk), kMostChunk);
+  chunk = std::max({chunk, longest / kMostSplit, longest * tasks / kMostItems});
+  if (weighted && p.mfma) // a whole task may have 3/2 of it
+    chunk = std::min<uint64_t>(chunk, kScoreBytes / (p.rows * 4u) * 2u / 3u);
+  chunk = (chunk + 63u) & ~uint64_t(63);
+  if (weighted && p.mfma && (chunk + chunk / 2u + 63u) / 64u * 64u * p.rows * 4u > kScoreBytes)
+    chunk -= 64u;
+  p.chunk = (uint32_t)chunk;
+  p.nsplit = longest <= chunk + chunk / 2u ? 1u : (uint32_t)((longest + chunk - 1u) / chunk);
   if (weighted) {
     // a call's pages are distinct: never more of them than the pool has
     uint64_t pages = a->page_indptr ? a->max_pages : (uint64_t)a->num_requests * a->max_pages;
@@ -550,12 +557,13 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   P.D = a->head_dim, P.ps = a->page_size, P.bt_stride = a->bt_stride;
   P.max_pages = a->max_pages, P.num_pages = (uint32_t)a->num_pages;
   P.q_dtype = a->q_dtype, P.o_dtype = a->o_dtype;
-  P.nsplit = plan.nsplit, P.least = plan.least;
+  P.nsplit = plan.nsplit, P.chunk = plan.chunk;
   const float dims = (float)(diff ? a->head_dim / 2u : a->head_dim);
   P.scale_log2 = (a->sm_scale != 0.f ? a->sm_scale : 1.0f / std::sqrt(dims)) *
                  1.4426950408889634f;
   P.w = a->weights, P.w_ps = a->w_page_stride, P.w_hs = a->w_head_stride;
   P.counted = a->counted, P.decay = a->decay;
+  P.w_vec = ((uintptr_t)a->weights & 15u) == 0 && a->w_page_stride % 4 == 0 && a->w_head_stride % 4 == 0;
   P.lam = a->lam, P.nw = a->norm_weight, P.eps = a->eps, P.mul = a->out_scale;
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
   P.scores = reinterpret_cast<float *>(ws), P.score_blocks = plan.score_blocks;
@@ -579,19 +587,20 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   uint32_t lds = 0;
   if (plan.mfma && !diff) {
     // the longest chunk's scores
-    const uint64_t even = (longest + P.nsplit - 1) / P.nsplit;
-    const uint64_t chunk = (std::max<uint64_t>(std::min<uint64_t>(even, longest), P.least) + 63) & ~uint64_t(63);
-    lds = (uint32_t)(chunk * P.rows * 4u);
+    const uint64_t most = (std::min<uint64_t>(longest, P.chunk + P.chunk / 2u) + 63u) & ~uint64_t(63);
+    lds = (uint32_t)(most * P.rows * 4u);
   }
   hipLaunchKernelGGL(fn, dim3(tasks, P.nsplit), dim3(kBlock), lds, s, P);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && P.nsplit > P.join_from) {
-    uint32_t by = P.G;
-    if (!diff) // two tokens a lane, fewer workgroups where the tasks are many
+    // few chunks: one workgroup has all of a task's outputs
+    const uint32_t outs = P.nsplit <= 16u ? 1u : P.G;
+    uint32_t by = outs;
+    if (!diff)
       by += (uint32_t)std::max<uint64_t>(
-          1, std::min<uint64_t>((longest + 2 * kJoin - 1) / (2 * kJoin), 4096u / tasks + 1u));
+          1, std::min<uint64_t>((longest + kTokens - 1) / kTokens, 4096u / tasks + 1u));
     hipLaunchKernelGGL(diff ? join_of<true>(P.D) : join_of<false>(P.D), dim3(tasks, by),
-                       dim3(kJoin), 0, s, P);
+                       dim3(kJoin), 0, s, P, outs);
     e = hipGetLastError();
   }
   if (e != hipSuccess)

@@ -28,7 +28,7 @@ struct MapParams {
   uint32_t R, Hq, Hkv, G, rows; // rows: maps per kv-head (G, or 2 G)
   uint32_t D, ps, bt_stride, max_pages, num_pages;
   uint32_t q_dtype, o_dtype;
-  uint32_t nsplit, least; // most chunks of a task; least tokens of one (a multiple of 64)
+  uint32_t nsplit, chunk; // most chunks of a task; tokens of one, about (map_chunk)
   uint32_t join_from;     // the join has tasks of more chunks than this to do
   float scale_log2;
   // weighted
@@ -36,6 +36,7 @@ struct MapParams {
   int64_t w_ps, w_hs;
   const int32_t *counted;
   float decay;
+  uint32_t w_vec;      // four slots' weights are one 16-byte access
   float *scores;       // [16-token block of the batch][kv-head][row][16]
   uint64_t score_blocks; // blocks it holds
   // difference
@@ -61,12 +62,11 @@ __device__ __forceinline__ int64_t map_row(const MapParams &P, uint32_t r) {
   return P.indptr ? (int64_t)P.indptr[r] : (int64_t)r * P.bt_stride;
 }
 
-// Tokens of a chunk of an n-token task: nsplit equal ones, none below `least`,
-// in multiples of 64.
+// Tokens of a chunk of an n-token task: all of them up to 3/2 P.chunk, else as many equal
+// chunks as P.chunk tokens each would make; in multiples of 64.
 __device__ __forceinline__ uint32_t map_chunk(const MapParams &P, uint32_t n) {
-  const uint32_t even = (uint32_t)(((uint64_t)n + P.nsplit - 1u) / P.nsplit);
-  const uint32_t c = even > P.least ? even : P.least;
-  return (c + 63u) & ~63u;
+  const uint32_t nch = n <= P.chunk + P.chunk / 2u ? 1u : (n + P.chunk - 1u) / P.chunk;
+  return ((n + nch - 1u) / nch + 63u) & ~63u;
 }
 
 // Score blocks of the requests before r (one wave or more; every lane takes part
@@ -100,6 +100,47 @@ __device__ __forceinline__ float map_load_q(const MapParams &P, int64_t i) {
   return P.q_dtype == SCHED_PD_F32   ? static_cast<const float *>(P.q)[i]
          : P.q_dtype == SCHED_PD_F16 ? (float)static_cast<const _Float16 *>(P.q)[i]
                                      : bf16_bits_to_f32(static_cast<const uint16_t *>(P.q)[i]);
+}
+
+// The weights of four tokens t .. t + 3 of a request (t a multiple of 4): their scores at s
+// (row g: s + 16 g floats), M and 1 / L of the rows in s_M, s_Li. Tokens from n on keep what
+// their slots hold.
+__device__ __forceinline__ void map_weights4(const MapParams &P, uint32_t h, uint32_t page,
+                                             uint32_t t, uint32_t n, int64_t have,
+                                             const float *s, const float *s_M,
+                                             const float *s_Li) {
+  typedef __attribute__((ext_vector_type(4))) float f32x4;
+  float *wp = P.w + (int64_t)page * P.w_ps + (int64_t)h * P.w_hs + t % P.ps;
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, old = {0.f, 0.f, 0.f, 0.f};
+  const bool vec = P.w_vec && t + 4u <= n;
+  if (vec) {
+    if ((int64_t)t < have)
+      old = *reinterpret_cast<const f32x4 *>(wp);
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (t + k < n && (int64_t)(t + k) < have)
+        old[k] = wp[k];
+  }
+#pragma unroll 4
+  for (uint32_t g = 0; g < P.rows; ++g) {
+    const f32x4 x = *reinterpret_cast<const f32x4 *>(s + g * 16u);
+    const float M = s_M[g], li = s_Li[g];
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      a[k] += __builtin_amdgcn_exp2f(x[k] - M) * li;
+  }
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k)
+    a[k] = (int64_t)(t + k) < have ? old[k] * P.decay + a[k] : a[k];
+  if (vec) {
+    *reinterpret_cast<f32x4 *>(wp) = a;
+  } else {
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k)
+      if (t + k < n)
+        wp[k] = a[k];
+  }
 }
 
 } // namespace schedpd

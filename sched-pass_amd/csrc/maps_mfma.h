@@ -535,16 +535,10 @@ __global__ void __launch_bounds__(NW * 64) maps_mfma(MapParams P) {
       map_store(P, ((int64_t)r * P.Hq + h * P.G + g) * D + j, n ? row_dim(g, j) * s_Li[g] : nan);
     }
     const int64_t have = P.counted ? (int64_t)P.counted[r] : (int64_t)n;
-    for (uint32_t t = tid; t < n; t += NT) {
+    for (uint32_t t = tid * 4u; t < n; t += NT * 4u) {
       const uint32_t page = (uint32_t)P.bt[T.row + t / P.ps];
-      if (page >= P.num_pages)
-        continue;
-      const float *s = s_sc + (t / 16u) * P.rows * 16u + (t & 15u);
-      float a = 0.f;
-      for (uint32_t g = 0; g < P.rows; ++g)
-        a += __builtin_amdgcn_exp2f(s[g * 16u] - s_M[g]) * s_Li[g];
-      float *wp = P.w + (int64_t)page * P.w_ps + (int64_t)h * P.w_hs + t % P.ps;
-      *wp = (int64_t)t < have ? *wp * P.decay + a : a;
+      if (page < P.num_pages)
+        map_weights4(P, h, page, t, n, have, s_sc + (t / 16u) * P.rows * 16u + (t & 15u), s_M, s_Li);
     }
   }
 }

@@ -21,14 +21,13 @@ using namespace schedpd;
 namespace {
 
 constexpr int kBlock = 256;
-#ifndef MANYT
-#define MANYT 2048
-#endif
-#ifndef NPER
-#define NPER 8
-#endif
-// From this many tokens on a lane group takes several of them, below one.
-constexpr uint32_t kManyTokens = MANYT, kTokensPer = NPER;
+// Workgroups of one token per lane group, W: below kOneToken of them each lane group takes one
+// token (a step of 256 tokens: 5.4 us, with two 6.6), from there on W / kFill of them, 4 to
+// 16. 4097 tokens of 18 rows of 64 dims (W 2341): one token 13.4 us, two 8.2, four 8.4,
+// eight 11.0, sixteen 15.7; 9 prompts of 301..2900 tokens, 48 rows of 128 dims (W 44000):
+// four 115, eight 108, sixteen 105. Non-temporal loads of the rows: 105 -> 99, but rows
+// that the projection has just written, as they come, 20.8 -> 25.2 (5000 tokens, 24 rows).
+constexpr uint32_t kOneToken = 2048, kFill = 1024, kLeastPer = 4, kMostPer = 16;
 
 struct RParams {
   const void *q, *k, *v;
@@ -620,26 +619,35 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
   for (const void *p : {a->q_weight, a->k_weight})
     vec = vec && (uintptr_t)p % (a->w_dtype == SCHED_PD_F32 ? 16 : 8) == 0;
   VecFn fn = nullptr;
-  const bool many = P.T >= kManyTokens;
+  Deal D{1u, 1u, 1.f / (float)a->head_dim};
   if (vec) {
-    const int lg = log2_of(a->head_dim / v), hlg = P.inter ? -1 : log2_of(a->rot_dim / 2u / v);
-    if (lg >= 0 && (P.inter || hlg >= 0))
-      fn = many ? vec_of<2>(a->dtype, lg, hlg) : vec_of<1>(a->dtype, lg, hlg);
-  }
-  if (fn) {
     const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u);
     const uint32_t groups = kBlock / (a->head_dim / v);
-    Deal D{1u, many ? kTokensPer : 1u, 1.f / (float)a->head_dim};
-    if (many) // as many tokens side by side, at most 8, as leave the fewest lane groups idle
-      for (uint32_t t = 1, best = ~0u; t <= 8; ++t) {
-        const uint32_t z = (t * rows + groups - 1u) / groups;
-        const uint32_t idle = (z * groups - t * rows) * 1000u / (z * groups);
-        if (idle < best)
-          best = idle, D.ts = t;
-      }
-    grid.z = (D.ts * rows + groups - 1u) / groups;
-    const uint64_t gy = ((uint64_t)most + D.ts * D.per - 1u) / (D.ts * D.per);
-    grid.y = (uint32_t)(gy < 65535u ? gy : 65535u);
+    auto across = [&](uint32_t t) { return (t * rows + groups - 1u) / groups; };
+    // as many tokens side by side, at most 8, as leave the fewest lane groups idle
+    uint32_t ts = 1, best = ~0u;
+    for (uint32_t t = 1; t <= 8; ++t) {
+      const uint32_t idle = (across(t) * groups - t * rows) * 1000u / (across(t) * groups);
+      if (idle < best)
+        best = idle, ts = t;
+    }
+    const uint64_t work = (uint64_t)P.T * across(ts) / ts;
+    const bool walk = work >= kOneToken;
+    const int lg = log2_of(a->head_dim / v), hlg = P.inter ? -1 : log2_of(a->rot_dim / 2u / v);
+    if (lg >= 0 && (P.inter || hlg >= 0))
+      fn = walk ? vec_of<2>(a->dtype, lg, hlg) : vec_of<1>(a->dtype, lg, hlg);
+    if (walk) {
+      const uint64_t per = work / kFill;
+      D.ts = ts;
+      D.per = (uint32_t)(per < kLeastPer ? kLeastPer : per > kMostPer ? kMostPer : per) & ~1u;
+    }
+    if (fn) {
+      grid.z = across(D.ts);
+      const uint64_t gy = ((uint64_t)most + D.ts * D.per - 1u) / (D.ts * D.per);
+      grid.y = (uint32_t)(gy < 65535u ? gy : 65535u);
+    }
+  }
+  if (fn) {
     hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, D);
   } else {
     auto every = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
