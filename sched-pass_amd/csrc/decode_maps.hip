@@ -198,16 +198,19 @@ __device__ __forceinline__ void join_rows(const MapParams &P, uint64_t item0, ui
 }
 
 // The join of what `maps_valu` and, for tasks of several chunks, maps_mfma left:
-// workgroup (task, y). y < outs: the outputs of q-heads y, y + outs, ...; from there on the
+// workgroup (task, y). y < outs: the output of q-head y (FEW: of all of them); from there on the
 // weights, kTokens tokens a workgroup and round. A dim's chunks are summed by kJoin / D lanes,
 // 8 loads in flight each, and their sums in order.
 constexpr uint32_t kTokens = 4 * kJoin;
 
-template <int D, bool DIFF>
+constexpr uint32_t FEWCH = 16; // chunks of a task up to which one workgroup has its outputs
+
+template <int D, bool DIFF, bool FEW>
 __global__ void __launch_bounds__(kJoin) maps_join(MapParams P, uint32_t outs) {
   constexpr uint32_t LANES = kJoin / D, NR = DIFF ? 2 : 1, CH = 64;
   __shared__ float s_M[kMostRows], s_Li[kMostRows];
   __shared__ float s_f[NR][CH], s_o[NR][LANES][D], s_sum[kJoin / 64];
+  __shared__ float s_w[kMostRows][FEWCH];
   const uint32_t tid = threadIdx.x, task = blockIdx.x;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const uint32_t n = map_tokens(P, r), len = map_chunk(P, n);
@@ -215,14 +218,73 @@ __global__ void __launch_bounds__(kJoin) maps_join(MapParams P, uint32_t outs) {
   if (nch <= P.join_from)
     return; // the stream has finished this task
   const uint64_t item0 = (uint64_t)task * P.nsplit;
-  if (blockIdx.y < outs) {
-    if (outs == 1u)
-      join_rows(P, item0, nch, 0u, P.rows, s_M, s_Li);
-    else
-      join_rows(P, item0, nch, blockIdx.y * NR, blockIdx.y * NR + NR, s_M, s_Li);
+  if (FEW && blockIdx.y == 0u) {
+    // a lane sums an element's few chunks: no workgroup-wide steps between the rows
+    join_rows(P, item0, nch, 0u, P.rows, s_M, s_Li);
+    __syncthreads();
+    if (tid < P.rows * FEWCH) {
+      const uint32_t g = tid / FEWCH, c = tid % FEWCH;
+      s_w[g][c] = c < nch ? __builtin_amdgcn_exp2f(P.ml[((item0 + c) * P.rows + g) * 2u] - s_M[g]) *
+                                s_Li[g]
+                          : 0.f;
+    }
+    __syncthreads();
+    const float *acc = P.acc + item0 * P.rows * D;
+    const uint32_t hop = P.rows * D;
+    auto joined = [&](uint32_t g, uint32_t j) __attribute__((always_inline)) {
+      float o = 0.f;
+      for (uint32_t c0 = 0; c0 < nch; c0 += 4u) {
+        float v[4];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+          v[u] = acc[(uint64_t)min(c0 + u, nch - 1u) * hop + g * D + j];
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+          o += c0 + u < nch ? v[u] * s_w[g][c0 + u] : 0.f;
+      }
+      return o;
+    };
+    const float nan = __builtin_nanf("");
+    if constexpr (!DIFF) {
+      for (uint32_t i = tid; i < P.rows * D; i += kJoin) {
+        const uint32_t g = i / D, j = i % D;
+        const float o = joined(g, j);
+        map_store(P, ((int64_t)r * P.Hq + h * P.G + g) * D + j, n ? o : nan);
+      }
+    } else {
+      const uint32_t lane = tid & 63u;
+      for (uint32_t g = tid >> 6; g < P.G; g += kJoin / 64) {
+        const uint32_t hq = h * P.G + g;
+        const float la = P.lam[hq];
+        float o[D / 64], ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const uint32_t j = lane + 64u * i;
+          o[i] = joined(2u * g, j) - la * joined(2u * g + 1u, j);
+          ss += o[i] * o[i];
+        }
+        float inv = P.mul;
+        if (P.nw) {
+#pragma unroll
+          for (int k = 32; k > 0; k >>= 1)
+            ss += __shfl_xor(ss, k);
+          inv *= rsqrtf(ss / (float)D + P.eps);
+        }
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const uint32_t j = lane + 64u * i;
+          map_store(P, ((int64_t)r * P.Hq + hq) * D + j,
+                    n ? o[i] * inv * (P.nw ? P.nw[j] : 1.f) : nan);
+        }
+      }
+    }
+    return;
+  }
+  if (!FEW && blockIdx.y < outs) {
+    join_rows(P, item0, nch, blockIdx.y * NR, blockIdx.y * NR + NR, s_M, s_Li);
     const uint32_t j = tid % D, part = tid / D;
-    for (uint32_t g = blockIdx.y; g < P.G; g += outs) {
-      const uint32_t g0 = g * NR, hq = h * P.G + g;
+    {
+      const uint32_t g = blockIdx.y, g0 = g * NR, hq = h * P.G + g;
       float o[NR] = {};
       for (uint32_t c0 = 0; c0 < nch; c0 += CH) {
         const uint32_t cnt = min(CH, nch - c0);
@@ -312,11 +374,11 @@ __global__ void __launch_bounds__(kJoin) maps_join(MapParams P, uint32_t outs) {
   }
 }
 
-template <bool DIFF> auto join_of(uint32_t d) {
-  return d == 32    ? maps_join<DIFF ? 64 : 32, DIFF>
-         : d == 64  ? maps_join<64, DIFF>
-         : d == 128 ? maps_join<128, DIFF>
-                    : maps_join<256, DIFF>;
+template <bool DIFF, bool FEW> auto join_of(uint32_t d) {
+  return d == 32    ? maps_join<DIFF ? 64 : 32, DIFF, FEW>
+         : d == 64  ? maps_join<64, DIFF, FEW>
+         : d == 128 ? maps_join<128, DIFF, FEW>
+                    : maps_join<256, DIFF, FEW>;
 }
 
 uint64_t up256(uint64_t x) { return (x + 255u) & ~uint64_t(255); }
@@ -466,10 +528,16 @@ template <int KV, int D, bool VT, bool DIFF> StreamFn mfma_rows(uint32_t rows) {
 #define W256 2
 #endif
 #ifndef W128
-#define W128 3
+#define W128 2
 #endif
-  constexpr int DEPTH = D == 256 ? (KV == kMapFp8 ? 2 : D256) : D == 128 ? (KV == kMapFp8 ? 3 : 2) : 4;
-  constexpr int WPE = D == 256 ? W256 : D == 128 ? W128 : 3;
+#ifndef D128
+#define D128 2
+#endif
+#ifndef W128F
+#define W128F 3
+#endif
+  constexpr int DEPTH = D == 256 ? (KV == kMapFp8 ? 2 : D256) : D == 128 ? (KV == kMapFp8 ? 3 : D128) : 4;
+  constexpr int WPE = D == 256 ? W256 : D == 128 ? (KV == kMapFp8 ? W128F : W128) : 3;
   return rows <= 4   ? maps_mfma<KV, D, VT, 4, DIFF, 4, DEPTH, WPE>
          : rows <= 8 ? maps_mfma<KV, D, VT, 8, DIFF, 4, DEPTH, WPE>
                      : maps_mfma<KV, D, VT, 16, DIFF, 4, DEPTH, WPE>;
@@ -594,13 +662,15 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && P.nsplit > P.join_from) {
     // few chunks: one workgroup has all of a task's outputs
-    const uint32_t outs = P.nsplit <= 16u ? 1u : P.G;
+    const bool few = P.nsplit <= FEWCH;
+    const uint32_t outs = few ? 1u : P.G;
     uint32_t by = outs;
     if (!diff)
       by += (uint32_t)std::max<uint64_t>(
           1, std::min<uint64_t>((longest + kTokens - 1) / kTokens, 4096u / tasks + 1u));
-    hipLaunchKernelGGL(diff ? join_of<true>(P.D) : join_of<false>(P.D), dim3(tasks, by),
-                       dim3(kJoin), 0, s, P, outs);
+    auto join = few ? (diff ? join_of<true, true>(P.D) : join_of<false, true>(P.D))
+                    : (diff ? join_of<true, false>(P.D) : join_of<false, false>(P.D));
+    hipLaunchKernelGGL(join, dim3(tasks, by), dim3(kJoin), 0, s, P, outs);
     e = hipGetLastError();
   }
   if (e != hipSuccess)

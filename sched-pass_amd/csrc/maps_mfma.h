@@ -107,7 +107,7 @@ __device__ __forceinline__ void map_issue_v(const MapParams &P, const MapTask &T
 // Head dim 256 keeps its query operands in LDS: 32 registers that two blocks in flight
 // need.
 #ifndef QL
-#define QL 256
+#define QL 512
 #endif
 constexpr bool map_q_lds(int d) { return d >= QL; }
 
