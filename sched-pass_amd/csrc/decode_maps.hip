@@ -462,23 +462,17 @@ bool mfma_applies(const SchedMapsArgs *a) {
 
 // How tasks are cut (map_chunk): into chunks of 8 tokens for each task of the call, between
 // kLeastChunk and kMostChunk, so that a few long tasks fill the card and many tasks stay
-// whole, but for the longest. Longer ones where a wide table would make more than kMostSplit
-// chunks of a task or kMostItems of the call; on the matrix cores a weighted chunk's
-// scores fit kScoreBytes of LDS.
-#ifndef LEASTC
-#define LEASTC 256
-#endif
-#ifndef MOSTC
-#define MOSTC 2048
-#endif
-#ifndef PERT
-#define PERT 8
-#endif
-#ifndef SCB
-#define SCB 40
-#endif
-constexpr uint64_t kLeastChunk = LEASTC, kMostChunk = MOSTC, kMostSplit = 128, kMostItems = 4096;
-constexpr uint32_t kScoreBytes = SCB << 10;
+// whole, but for the longest (a split task costs its partials and the join). In us, bf16,
+// 32 / 8 heads of 128, at 4, 8 and 16 tokens a task: 16 x 2048 tokens 33.0 / 31.0 / 34.0, 32
+// x 2048 56.9 / 47.7 / 47.5, differential 48 requests of 200..2900 71.4 / 65.0 / 65.3; one
+// request of 1000 with kLeastChunk 256 13.6, with 512 15.5. Longer chunks where a table would
+// make more than kMostSplit of a task (one request of 100003 tokens: 64 of them 79.3, 96 82.2,
+// 128 84.4: more than one round of workgroups) or kMostItems of the call. On the matrix
+// cores a weighted chunk's scores fit kScoreBytes of LDS (64 lognormal contexts up to 4000:
+// 32 KB 81.7, 40 77.5, 48 83.5; 64 x 2048: 32 KB cut in two, 107, 40 90.3).
+constexpr uint64_t kChunkPerTask = 8, kLeastChunk = 256, kMostChunk = 2048;
+constexpr uint64_t kMostSplit = 64, kMostItems = 4096;
+constexpr uint32_t kScoreBytes = 40u << 10;
 
 Plan plan_of(const SchedMapsArgs *a) {
   Plan p{};
@@ -487,7 +481,7 @@ Plan plan_of(const SchedMapsArgs *a) {
   const bool weighted = a->op == SCHED_MAPS_WEIGHTED;
   p.mfma = mfma_applies(a);
   p.rows = a->num_q_heads / a->num_kv_heads * (weighted ? 1u : 2u);
-  uint64_t chunk = std::min(std::max(PERT * tasks, kLeastChunk), kMostChunk);
+  uint64_t chunk = std::min(std::max(kChunkPerTask * tasks, kLeastChunk), kMostChunk);
   chunk = std::max({chunk, longest / kMostSplit, longest * tasks / kMostItems});
   if (weighted && p.mfma) // a whole task may have 3/2 of it
     chunk = std::min<uint64_t>(chunk, kScoreBytes / (p.rows * 4u) * 2u / 3u);
@@ -519,25 +513,15 @@ template <typename T> StreamFn valu_of(uint32_t d, bool diff) {
   }
 }
 
-// Blocks in flight per wave and waves per SIMD they leave room for.
+// Blocks in flight per wave and the waves per SIMD they leave room for. Head dim 128 of 16
+// bits at three waves spills 4 registers (64 lognormal contexts 87 us, at two 77.5); two
+// blocks of 256 dims spill 44 at two waves, and at one wave without spills take 52.3 us
+// where one block at two waves takes 48.4 (32771 tokens, the keys of the next block
+// under way while a block's values are multiplied).
 template <int KV, int D, bool VT, bool DIFF> StreamFn mfma_rows(uint32_t rows) {
-#ifndef D256
-#define D256 1
-#endif
-#ifndef W256
-#define W256 2
-#endif
-#ifndef W128
-#define W128 2
-#endif
-#ifndef D128
-#define D128 2
-#endif
-#ifndef W128F
-#define W128F 3
-#endif
-  constexpr int DEPTH = D == 256 ? (KV == kMapFp8 ? 2 : D256) : D == 128 ? (KV == kMapFp8 ? 3 : D128) : 4;
-  constexpr int WPE = D == 256 ? W256 : D == 128 ? (KV == kMapFp8 ? W128F : W128) : 3;
+  constexpr bool FP8 = KV == kMapFp8;
+  constexpr int DEPTH = D == 256 ? (FP8 ? 2 : 1) : D == 128 ? (FP8 ? 3 : 2) : 4;
+  constexpr int WPE = D == 256 || (D == 128 && !FP8) ? 2 : 3;
   return rows <= 4   ? maps_mfma<KV, D, VT, 4, DIFF, 4, DEPTH, WPE>
          : rows <= 8 ? maps_mfma<KV, D, VT, 8, DIFF, 4, DEPTH, WPE>
                      : maps_mfma<KV, D, VT, 16, DIFF, 4, DEPTH, WPE>;

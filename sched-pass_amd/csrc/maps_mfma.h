@@ -104,17 +104,10 @@ __device__ __forceinline__ void map_issue_v(const MapParams &P, const MapTask &T
   }
 }
 
-// Head dim 256 keeps its query operands in LDS: 32 registers that two blocks in flight
-// need.
-#ifndef QL
-#define QL 512
-#endif
-constexpr bool map_q_lds(int d) { return d >= QL; }
-
 template <int D> struct MapState {
   float m, l;
   f32x4_t acc[D / 16];
-  bf16x8_t q[map_q_lds(D) ? 1 : D / 32];
+  bf16x8_t q[D / 32];
 };
 
 // The A operand of dim block blk: 4 tokens of one dim. fp8 blocks come as one dword of
@@ -149,8 +142,7 @@ constexpr float kF16P = 4096.f; // fp16 probabilities travel times this
 template <int KV, int D, bool VT, bool DIFF, typename F>
 __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T, MapState<D> &S,
                                             const BlockRegs<KV, D> &B, uint32_t blk_in_chunk,
-                                            const u32x4_t *s_q, float *s_sc, uint32_t c16,
-                                            uint32_t g4, F next_k) {
+                                            float *s_sc, uint32_t c16, uint32_t g4, F next_k) {
   typedef BlockRegs<KV, D> R;
   u32x4_t kk[R::NK];
 #pragma unroll
@@ -159,8 +151,6 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
   if constexpr (R::NK > 1)
     k_operands(kk);
   f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
-  if constexpr (map_q_lds(D)) // read anew for each block, not kept in registers
-    asm volatile("" : "+v"(s_q));
 #pragma unroll
   for (int kb = 0; kb < D / 32; ++kb) {
     bf16x8_t a;
@@ -172,10 +162,7 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
       const u32x2_t hi = fp8x4_to_bf16x4((kb & 1) ? raw.w : raw.y);
       a = __builtin_bit_cast(bf16x8_t, u32x4_t{lo.x, lo.y, hi.x, hi.y});
     }
-    if constexpr (map_q_lds(D))
-      sc = mfma_qk<KV == kMapF16>(a, __builtin_bit_cast(bf16x8_t, s_q[64 * kb]), sc);
-    else
-      sc = mfma_qk<KV == kMapF16>(a, S.q[kb], sc);
+    sc = mfma_qk<KV == kMapF16>(a, S.q[kb], sc);
   }
   const float ks = KV == kMapFp8 ? P.scale_log2 * B.ks : P.scale_log2, vs = B.vs;
   next_k();
@@ -327,8 +314,7 @@ __device__ __forceinline__ MapBlock in_pool(const MapParams &P, MapBlock b) {
 // last block into unused slots.
 template <int KV, int D, bool VT, bool DIFF, int NW, int DEPTH>
 __device__ __forceinline__ void map_stream(const MapParams &P, const MapTask &T, MapState<D> &S,
-                                           const u32x4_t *s_q, float *s_sc, uint32_t c16,
-                                           uint32_t g4) {
+                                           float *s_sc, uint32_t c16, uint32_t g4) {
   const int cnt = T.nblk > T.w ? (int)((T.nblk - T.w + NW - 1) / NW) : 0;
   if (cnt <= 0)
     return;
@@ -348,8 +334,8 @@ __device__ __forceinline__ void map_stream(const MapParams &P, const MapTask &T,
 #pragma unroll
     for (int s = 0; s < DEPTH; ++s) {
       const MapBlock b = in_pool(P, next[s]);
-      map_compute<KV, D, VT, DIFF>(P, T, S, buf[s], T.w + NW * (uint32_t)(j + s), s_q, s_sc, c16,
-                                   g4, [&]() __attribute__((always_inline)) {
+      map_compute<KV, D, VT, DIFF>(P, T, S, buf[s], T.w + NW * (uint32_t)(j + s), s_sc, c16, g4,
+                                   [&]() __attribute__((always_inline)) {
                                      map_issue_k<KV, D>(P, T, b, buf[s]);
                                    });
       map_issue_v<KV, D, VT>(P, T, b, buf[s]);
@@ -362,8 +348,8 @@ __device__ __forceinline__ void map_stream(const MapParams &P, const MapTask &T,
       if (j + s < cnt) {
         const bool more = j + DEPTH + s < cnt;
         const MapBlock b = in_pool(P, next[s]);
-        map_compute<KV, D, VT, DIFF>(P, T, S, buf[s], T.w + NW * (uint32_t)(j + s), s_q, s_sc, c16,
-                                     g4, [&]() __attribute__((always_inline)) {
+        map_compute<KV, D, VT, DIFF>(P, T, S, buf[s], T.w + NW * (uint32_t)(j + s), s_sc, c16, g4,
+                                     [&]() __attribute__((always_inline)) {
                                        if (more)
                                          map_issue_k<KV, D>(P, T, b, buf[s]);
                                      });
@@ -384,7 +370,6 @@ __global__ void __launch_bounds__(NW * 64) maps_mfma(MapParams P) {
   __shared__ float s_acc[NW][GMAX][D];
   __shared__ float s_m[NW][GMAX], s_l[NW][GMAX];
   __shared__ float s_M[GMAX], s_Li[GMAX];
-  __shared__ u32x4_t s_q[map_q_lds(D) ? D / 32 * 64 : 1];
   extern __shared__ float s_sc[];
   const uint32_t tid = threadIdx.x, lane = tid & 63u;
   const uint32_t w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -435,15 +420,10 @@ __global__ void __launch_bounds__(NW * 64) maps_mfma(MapParams P) {
     if (c16 < P.rows && (!DIFF || (d0 >= D / 2) == ((c16 & 1u) != 0u)))
       qv = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(P.q) +
                                               ((int64_t)r * P.Hq + hq) * D + d0);
-    if constexpr (map_q_lds(D)) // every wave has the same operands
-      s_q[64 * kb + lane] = qv;
-    else
-      S.q[kb] = __builtin_bit_cast(bf16x8_t, qv);
+    S.q[kb] = __builtin_bit_cast(bf16x8_t, qv);
   }
-  if constexpr (map_q_lds(D))
-    __syncthreads();
 
-  map_stream<KV, D, VT, DIFF, NW, DEPTH>(P, T, S, s_q + lane, s_sc, c16, g4);
+  map_stream<KV, D, VT, DIFF, NW, DEPTH>(P, T, S, s_sc, c16, g4);
 
   const float lt = sum_rows(S.l);
   if (c16 < P.rows) {
