@@ -1,14 +1,17 @@
 // evict.hip -- eviction by accumulated attention weight (sched_kv_evict): per
 // (request, kv-head) the m heaviest of n cached tokens stay, in their order, in slots
-// 0 .. m-1. Two launches:
+// 0 .. m-1.
 //   select: one workgroup per (request, kv-head) finds the weight T of the last kept
 //           token by radix (the bits of a weight as an unsigned number that orders
-//           like it, eight at a time from the top: a histogram, then the digit in which
-//           the wanted rank falls), then walks the tokens once in order, keeping those
-//           above T and the first ties;
-//   move:   one workgroup per (request, kv-head, keys or values) copies the kept rows
-//           down, a batch of rows at a time. A row's new slot is never behind its old
-//           one, so a batch may be written once it and every batch before it have been read.
+//           like it, eight at a time from the highest that differ: a histogram, then the
+//           digit in which the wanted rank falls), then keeps, in order, those above T
+//           and the first ties. Its keys stay in registers, each weight is read once.
+//   move:   one workgroup per (request, kv-head, keys or values, part of the row) copies
+//           the kept rows down, a round of rows at a time. A row's new slot is never
+//           behind its old one, so what a round overwrites are rows of its own or of
+//           earlier rounds: it may be written once all of it has been read, with the next
+//           round's reads already under way.
+//   fp8: a third launch stores the pages' new scales, behind the last read of the old ones.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,6 +40,7 @@ struct EParams {
   uint32_t R, Hkv, D, ps, bt_stride, max_pages, max_keep, new_pages;
   uint32_t sink, recent;
   uint32_t num_pages;
+  uint32_t ps_magic; // ceil(2^32 / ps): t / ps for t up to 2^24
 };
 
 struct Req {
@@ -64,13 +68,77 @@ __device__ __forceinline__ uint32_t order_bits(float f) {
   return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kSelect = 1024;
 constexpr int kVmcnt0 = 0x0F70; // s_waitcnt vmcnt(0), the other counters at their maxima
 
-__global__ void __launch_bounds__(kSelect) evict_select(EParams P) {
+__device__ __forceinline__ uint32_t div_ps(const EParams &P, uint32_t t) {
+  return __umulhi(t, P.ps_magic);
+}
+
+// Inclusive sums of x over the workgroup's lanes in order; *all: the sum of all.
+template <int NT>
+__device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *s_wave, uint32_t *all) {
+  const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(x, o);
+    x += lane >= (uint32_t)o ? y : 0u;
+  }
+  __syncthreads(); // s_wave's previous values have been read
+  if (lane == 63u)
+    s_wave[wave] = x;
+  __syncthreads();
+  uint32_t before = 0u, sum = 0u;
+#pragma unroll
+  for (uint32_t k = 0; k < NT / 64; ++k) {
+    before += k < wave ? s_wave[k] : 0u;
+    sum += s_wave[k];
+  }
+  *all = sum;
+  return x + before;
+}
+
+// The digit of s_hist (256 counts) in which the left-th largest falls, and how many lie
+// above it; by the first wave, four digits a lane.
+__device__ __forceinline__ void pick_digit(const uint32_t *s_hist, uint32_t left, uint32_t *s_pick) {
+  const uint32_t lane = threadIdx.x;
+  if (lane >= 64u)
+    return;
+  // lane 0 has the highest digits
+  uint32_t c[4], sum = 0u;
+#pragma unroll
+  for (uint32_t k = 0; k < 4; ++k) {
+    c[k] = s_hist[255u - (4u * lane + k)];
+    sum += c[k];
+  }
+  uint32_t incl = sum;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t y = __shfl_up(incl, o);
+    incl += lane >= (uint32_t)o ? y : 0u;
+  }
+  uint32_t above = incl - sum;
+  if (above < left && left <= incl) {
+#pragma unroll
+    for (uint32_t k = 0; k < 4; ++k) {
+      if (above < left && left <= above + c[k]) {
+        s_pick[0] = 255u - (4u * lane + k);
+        s_pick[1] = above;
+        s_pick[2] = c[k];
+      }
+      above += c[k];
+    }
+  }
+}
+
+// NT lanes with KREG tokens each in registers, a stretch (its token t0 + i NT + lane). A
+// request of one stretch is read once; a longer one stretch by stretch for each digit.
+template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(EParams P) {
+  constexpr uint32_t NW = NT / 64, SPAN = NT * KREG;
+  constexpr uint32_t E = (KREG * NW + NT - 1) / NT; // counts of a lane in a scan
+  static_assert(KREG <= 32, "a bit for each token of a lane");
   __shared__ uint32_t s_hist[256];
-  __shared__ uint32_t s_wave[2][kSelect / 64];
-  __shared__ uint32_t s_pick[2];
+  __shared__ uint32_t s_cnt[KREG * NW];
+  __shared__ uint32_t s_wave[NW], s_pick[3], s_lo[NW], s_hi[NW];
   __shared__ uint32_t s_bad;
   const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
   const uint32_t task = blockIdx.x, r = task / P.Hkv, h = task % P.Hkv;
@@ -81,12 +149,12 @@ __global__ void __launch_bounds__(kSelect) evict_select(EParams P) {
   __syncthreads();
   const uint32_t pages = (uint32_t)((q.n + (uint64_t)P.ps - 1u) / P.ps);
   if (q.ok)
-    for (uint32_t b = tid; b < pages; b += kSelect)
+    for (uint32_t b = tid; b < pages; b += NT)
       if ((uint32_t)P.bt[q.row + b] >= P.num_pages)
         s_bad = 1u;
   __syncthreads();
   if (s_bad) { // nothing of this request is touched
-    for (uint32_t j = tid; j < P.max_keep; j += kSelect)
+    for (uint32_t j = tid; j < P.max_keep; j += NT)
       kept[j] = -1;
     if (tid == 0 && P.errors)
       atomicAdd(P.errors, 1u);
@@ -95,96 +163,191 @@ __global__ void __launch_bounds__(kSelect) evict_select(EParams P) {
   const uint32_t recent = min(q.m, P.recent), sink = min(P.sink, q.m - recent);
   const uint32_t lo = sink, hi = q.n - recent; // the tokens that compete
   const uint32_t want = q.m - recent - sink;
-  auto weight = [&](uint32_t t) {
-    return P.w[(int64_t)P.bt[q.row + t / P.ps] * P.w_ps + (int64_t)h * P.w_hs + t % P.ps];
+  const bool cut = q.m < q.n, one = q.n <= SPAN;
+  const float *w0 = P.w + (int64_t)h * P.w_hs;
+
+  float x[KREG];
+  auto load = [&](uint32_t t0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < KREG; ++i) {
+      const uint32_t t = t0 + (uint32_t)i * NT + tid;
+      x[i] = 0.f;
+      if (t < q.n) {
+        const uint32_t b = div_ps(P, t);
+        x[i] = w0[(int64_t)P.bt[q.row + b] * P.w_ps + (t - b * P.ps)];
+      }
+    }
   };
-  // the want-th largest key, digit by digit; `left` of its equals are kept
+  load(0);
   uint32_t T = 0u, left = 0u;
-  if (q.m < q.n && want > 0u) {
-    left = want;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256u)
-        s_hist[tid] = 0u;
-      __syncthreads();
-      for (uint32_t t = lo + tid; t < hi; t += kSelect) {
-        const uint32_t key = order_bits(weight(t));
-        if (shift == 24 || (key >> (shift + 8)) == (T >> (shift + 8)))
-          atomicAdd(&s_hist[(key >> shift) & 255u], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t d = 255u, above = 0u;
-        while (d > 0u && above + s_hist[d] < left) {
-          above += s_hist[d];
-          --d;
+  if (cut && want > 0u) {
+    // the highest bit in which the competing keys differ
+    uint32_t kmin = ~0u, kmax = 0u;
+    for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
+      if (t0 > 0u)
+        load(t0);
+#pragma unroll
+      for (int i = 0; i < KREG; ++i) {
+        const uint32_t t = t0 + (uint32_t)i * NT + tid;
+        if (t >= lo && t < hi) {
+          const uint32_t key = order_bits(x[i]);
+          kmin = min(kmin, key);
+          kmax = max(kmax, key);
         }
-        s_pick[0] = d;
-        s_pick[1] = above;
       }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+      kmin = min(kmin, (uint32_t)__shfl_xor(kmin, o));
+      kmax = max(kmax, (uint32_t)__shfl_xor(kmax, o));
+    }
+    if (lane == 0) {
+      s_lo[wave] = kmin;
+      s_hi[wave] = kmax;
+    }
+    __syncthreads();
+#pragma unroll
+    for (uint32_t k = 0; k < NW; ++k) {
+      kmin = min(kmin, s_lo[k]);
+      kmax = max(kmax, s_hi[k]);
+    }
+    const uint32_t differ = kmin ^ kmax;
+    int top = differ ? 32 - __builtin_clz(differ) : 0; // the bits [0, top) differ
+    T = top < 32 ? kmax >> top << top : 0u;
+    left = want;
+    while (top > 0) {
+      const int shift = top > 8 ? top - 8 : 0;
+      const uint32_t mask = (1u << (top - shift)) - 1u; // a digit of at most eight bits
+      for (uint32_t k = tid; k < 256u; k += NT)
+        s_hist[k] = 0u;
+      __syncthreads();
+      for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
+        if (!one)
+          load(t0);
+#pragma unroll
+        for (int i = 0; i < KREG; ++i) {
+          if (t0 + (uint32_t)i * NT >= q.n)
+            break;
+          const uint32_t t = t0 + (uint32_t)i * NT + tid;
+          const uint32_t key = order_bits(x[i]);
+          if (t >= lo && t < hi && (top >= 32 || (key >> top) == (T >> top)))
+            atomicAdd(&s_hist[(key >> shift) & mask], 1u);
+        }
+      }
+      __syncthreads();
+      pick_digit(s_hist, left, s_pick);
       __syncthreads();
       T |= s_pick[0] << shift;
       left -= s_pick[1];
+      top = shift;
+      // the whole digit is kept: everything from T on, whatever its lower bits
+      if (s_pick[2] == left && T > 0u) {
+        T -= 1u;
+        left = 0u;
+        top = 0;
+      }
       __syncthreads();
     }
   }
-  // one walk in order: the kept tokens' slots, and their weights moved along
-  uint32_t base = 0u, ties = 0u;
-  for (uint32_t t0 = 0; t0 < q.n; t0 += kSelect) {
-    const uint32_t t = t0 + tid;
-    float x = 0.f;
-    bool always = false, above = false, tie = false;
-    if (t < q.n) {
-      x = weight(t);
-      always = t < lo || t >= hi || q.m == q.n;
-      if (!always && want > 0u) {
-        const uint32_t key = order_bits(x);
-        above = key > T;
-        tie = key == T;
+
+  // exclusive sums, in token order, of the stretch's counts per (i, wave); returns their sum
+  auto scan = [&](uint32_t t0) __attribute__((always_inline)) {
+    __syncthreads();
+    uint32_t c[E], sum = 0u, all;
+#pragma unroll
+    for (uint32_t k = 0; k < E; ++k) {
+      const uint32_t e = tid * E + k;
+      c[k] = e < KREG * NW && t0 + e / NW * NT < q.n ? s_cnt[e] : 0u;
+      sum += c[k];
+    }
+    uint32_t at = block_scan<NT>(sum, s_wave, &all) - sum;
+#pragma unroll
+    for (uint32_t k = 0; k < E; ++k) {
+      const uint32_t e = tid * E + k;
+      if (e < KREG * NW)
+        s_cnt[e] = at;
+      at += c[k];
+    }
+    __syncthreads();
+    return all;
+  };
+  uint32_t base = 0u, seen = 0u; // kept tokens and ties of the stretches before
+  const unsigned long long below = (1ull << lane) - 1ull;
+  for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
+    if (!one)
+      load(t0);
+    uint32_t stay = 0u; // bit i: this lane's token i is kept
+    if (cut && left > 0u) { // the first `left` tokens of weight T are
+#pragma unroll
+      for (int i = 0; i < KREG; ++i) {
+        if (t0 + (uint32_t)i * NT >= q.n)
+          break;
+        const uint32_t t = t0 + (uint32_t)i * NT + tid;
+        const unsigned long long b = __ballot(t >= lo && t < hi && order_bits(x[i]) == T);
+        if (lane == 0)
+          s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
+      }
+      const uint32_t all = scan(t0);
+#pragma unroll
+      for (int i = 0; i < KREG; ++i) {
+        if (t0 + (uint32_t)i * NT >= q.n)
+          break;
+        const uint32_t t = t0 + (uint32_t)i * NT + tid;
+        const bool tie = t >= lo && t < hi && order_bits(x[i]) == T;
+        const unsigned long long b = __ballot(tie);
+        if (tie && seen + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below) < left)
+          stay |= 1u << i;
+      }
+      seen += all;
+      __syncthreads();
+    }
+#pragma unroll
+    for (int i = 0; i < KREG; ++i) {
+      if (t0 + (uint32_t)i * NT >= q.n)
+        break;
+      const uint32_t t = t0 + (uint32_t)i * NT + tid;
+      if (t < q.n && (!cut || t < lo || t >= hi || (want > 0u && order_bits(x[i]) > T)))
+        stay |= 1u << i;
+      const unsigned long long b = __ballot((stay >> i) & 1u);
+      if (lane == 0)
+        s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
+    }
+    // in place: every lane has this stretch's weights before one is overwritten; those of
+    // later stretches lie behind every slot that is written now
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    const uint32_t all = scan(t0);
+#pragma unroll
+    for (int i = 0; i < KREG; ++i) {
+      if (t0 + (uint32_t)i * NT >= q.n)
+        break;
+      const uint32_t t = t0 + (uint32_t)i * NT + tid;
+      const bool in = (stay >> i) & 1u;
+      const unsigned long long b = __ballot(in);
+      const uint32_t at = base + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below);
+      if (in && at < q.m) {
+        kept[at] = (int32_t)t;
+        if (t != at || P.wo != P.w) {
+          const uint32_t d = div_ps(P, at);
+          P.wo[(int64_t)P.bt[q.row + d] * P.w_ps + (int64_t)h * P.w_hs + (at - d * P.ps)] = x[i];
+        }
       }
     }
-    // in place, another wave writes a slot of this stretch after the barriers below
-    __builtin_amdgcn_s_waitcnt(kVmcnt0);
-    const unsigned long long mt = __ballot(tie);
-    if (lane == 0)
-      s_wave[0][wave] = (uint32_t)__popcll(mt);
-    __syncthreads();
-    uint32_t before = ties + (uint32_t)__popcll(mt & ((1ull << lane) - 1ull)), all = 0u;
-    for (uint32_t k = 0; k < kSelect / 64; ++k) {
-      before += k < wave ? s_wave[0][k] : 0u;
-      all += s_wave[0][k];
-    }
-    const bool in = always || above || (tie && before < left);
-    const unsigned long long mk = __ballot(in);
-    if (lane == 0)
-      s_wave[1][wave] = (uint32_t)__popcll(mk);
-    __syncthreads();
-    uint32_t at = base + (uint32_t)__popcll(mk & ((1ull << lane) - 1ull)), some = 0u;
-    for (uint32_t k = 0; k < kSelect / 64; ++k) {
-      at += k < wave ? s_wave[1][k] : 0u;
-      some += s_wave[1][k];
-    }
-    // every weight of this stretch has been read: a slot behind it is never written
-    if (in && at < q.m) {
-      kept[at] = (int32_t)t;
-      if (t != at || P.wo != P.w)
-        P.wo[(int64_t)P.bt[q.row + at / P.ps] * P.w_ps + (int64_t)h * P.w_hs + at % P.ps] = x;
-    }
-    base += some;
-    ties += all;
+    base += all;
     __syncthreads();
   }
-  for (uint32_t j = q.m + tid; j < P.max_keep; j += kSelect)
+  for (uint32_t j = q.m + tid; j < P.max_keep; j += NT)
     kept[j] = -1;
   // fp8: the new scales of the pages that hold the kept tokens
-  if (P.new_scale != nullptr && q.m < q.n) {
+  if (P.new_scale != nullptr && cut) {
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
     float *ns = P.new_scale + (int64_t)task * 2 * P.new_pages;
-    for (uint32_t b = tid; b * P.ps < q.m; b += kSelect) {
+    for (uint32_t b = tid; b * P.ps < q.m; b += NT) {
       float mk = 0.f, mv = 0.f;
       const uint32_t end = min(q.m, (b + 1u) * P.ps);
       for (uint32_t j = b * P.ps; j < end; ++j) {
         const int64_t si =
-            ((int64_t)P.bt[q.row + (uint32_t)kept[j] / P.ps] * P.Hkv + h) * P.scale_stride;
+            ((int64_t)P.bt[q.row + div_ps(P, (uint32_t)kept[j])] * P.Hkv + h) * P.scale_stride;
         mk = fmaxf(mk, P.ks[si]);
         mv = fmaxf(mv, P.vs[si]);
       }
@@ -192,6 +355,18 @@ __global__ void __launch_bounds__(kSelect) evict_select(EParams P) {
       ns[P.new_pages + b] = mv;
     }
   }
+}
+
+// Makes the compiler wait for a load into x here.
+__device__ __forceinline__ void hold(uint4 &x) {
+  asm volatile("" : "+v"(x.x), "+v"(x.y), "+v"(x.z), "+v"(x.w) : : "memory");
+}
+__device__ __forceinline__ void hold(uint32_t &x) { asm volatile("" : "+v"(x) : : "memory"); }
+__device__ __forceinline__ void hold(uint16_t &x) { asm volatile("" : "+v"(x) : : "memory"); }
+__device__ __forceinline__ void hold(uint8_t &x) {
+  uint32_t y = x;
+  asm volatile("" : "+v"(y) : : "memory");
+  x = (uint8_t)y;
 }
 
 // One e4m3 code from a page of scale s in a page of scale `to` (inv = 1 / to).
@@ -203,15 +378,22 @@ __device__ __forceinline__ uint32_t recode(uint32_t c, float s, float inv) {
 }
 
 constexpr int kMove = 512;
+constexpr uint32_t kStage = 2048; // rows whose places are in LDS at a time
 
 // U: the unit a row is moved in (16 bytes where rows are contiguous and aligned, else
-// one element); a row is `units` of them, unit_step bytes apart.
+// one element); a row is `units` of them, k_step / v_step bytes apart, `part` of them this
+// workgroup's.
 template <typename U, bool FP8>
-__global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, int64_t k_step,
-                                                    int64_t v_step, uint32_t eb) {
-  const uint32_t tid = threadIdx.x;
-  const uint32_t task = blockIdx.x >> 1;
-  const bool vals = (blockIdx.x & 1u) != 0u;
+__global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, uint32_t part,
+                                                    int64_t k_step, int64_t v_step, uint32_t eb) {
+  constexpr int N = 4; // units of a lane and round
+  // where a row comes from (-1: it stays) and goes to; fp8: its old scale, the new one's inverse
+  __shared__ int64_t s_from[kStage], s_to[kStage];
+  __shared__ float s_old[FP8 ? kStage : 1], s_inv[FP8 ? kStage : 1];
+  const uint32_t tid = threadIdx.x, tasks2 = 2u * P.R * P.Hkv;
+  const uint32_t which = blockIdx.x % tasks2, first = blockIdx.x / tasks2 * part;
+  const uint32_t task = which >> 1;
+  const bool vals = (which & 1u) != 0u;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const Req q = req_of(P, r);
   const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
@@ -219,62 +401,89 @@ __global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, i
     return;
   uint8_t *pool = vals ? P.v + (int64_t)h * P.vhs * eb : P.k + (int64_t)h * P.khs * eb;
   const int64_t ps_b = (vals ? P.vps : P.kps) * eb, ts_b = (vals ? P.vts : P.kts) * eb;
-  const int64_t step = vals ? v_step : k_step;
-  float *scale = vals ? P.vs : P.ks;
+  const float *scale = vals ? P.vs : P.ks;
   const float *ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
-  // kUnits units a lane and round
-  constexpr int kUnits = 4;
-  const uint64_t total = (uint64_t)q.m * units;
-  for (uint64_t u0 = 0; u0 < total; u0 += (uint64_t)kMove * kUnits) {
-    U x[kUnits];
-    uint8_t *to[kUnits];
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i) {
-      const uint64_t u = u0 + (uint64_t)i * kMove + tid;
-      to[i] = nullptr;
-      if (u >= total)
-        continue;
-      const uint32_t j = (uint32_t)(u / units), e = (uint32_t)(u % units);
-      const uint32_t src = (uint32_t)kept[j];
-      const int64_t sp = P.bt[q.row + src / P.ps], dp = P.bt[q.row + j / P.ps];
+  const uint32_t e = first + tid % part, rr = tid / part, rows = kMove / part;
+  const bool active = rr < rows && e < units;
+  const int64_t off = (int64_t)e * (vals ? v_step : k_step);
+  const uint32_t round = rows * N;
+
+  for (uint32_t j0 = 0; j0 < q.m; j0 += kStage) {
+    const uint32_t cnt = min(kStage, q.m - j0);
+    __syncthreads(); // the previous stage's places have been used
+    for (uint32_t i = tid; i < cnt; i += kMove) {
+      const uint32_t j = j0 + i, src = (uint32_t)kept[j];
+      const uint32_t sb = div_ps(P, src), db = div_ps(P, j);
+      const int64_t sp = P.bt[q.row + sb], dp = P.bt[q.row + db];
       bool moves = src != j;
-      float s = 0.f, inv = 0.f;
       if constexpr (FP8) {
-        s = scale[(sp * P.Hkv + h) * P.scale_stride];
-        const float n = ns[j / P.ps];
-        if (s != n) {
-          moves = true;
-          inv = n > 0.f ? 1.f / n : 0.f;
-        } else {
-          s = 0.f; // the codes stay
-        }
+        const float was = scale[(sp * P.Hkv + h) * P.scale_stride], now = ns[db];
+        s_old[i] = was;
+        s_inv[i] = was != now ? 1.f / now : 0.f; // 0: the codes stay
+        moves = moves || was != now;
       }
-      if (!moves)
-        continue;
-      x[i] = *reinterpret_cast<const U *>(pool + sp * ps_b + (int64_t)(src % P.ps) * ts_b +
-                                          (int64_t)e * step);
-      if constexpr (FP8) {
-        if (s != 0.f || inv != 0.f) {
-          U y = x[i];
-          uint8_t *b = reinterpret_cast<uint8_t *>(&y);
-          for (uint32_t k = 0; k < sizeof(U); ++k)
-            b[k] = (uint8_t)recode(b[k], s, inv);
-          x[i] = y;
-        }
-      }
-      to[i] = pool + dp * ps_b + (int64_t)(j % P.ps) * ts_b + (int64_t)e * step;
+      s_from[i] = moves ? sp * ps_b + (int64_t)(src - sb * P.ps) * ts_b : -1;
+      s_to[i] = dp * ps_b + (int64_t)(j - db * P.ps) * ts_b;
     }
-    __builtin_amdgcn_s_waitcnt(kVmcnt0);
-    __syncthreads(); // this round's rows have all been read
-#pragma unroll
-    for (int i = 0; i < kUnits; ++i)
-      if (to[i] != nullptr)
-        *reinterpret_cast<U *>(to[i]) = x[i];
-  }
-  if constexpr (FP8) {
     __syncthreads();
-    for (uint32_t b = tid; b * P.ps < q.m; b += kMove)
-      scale[((int64_t)P.bt[q.row + b] * P.Hkv + h) * P.scale_stride] = ns[b];
+    U x[N], nx[N];
+    auto fetch = [&](uint32_t k0) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t k = k0 + (uint32_t)i * rows + rr;
+        nx[i] = U{};
+        if (active && k < cnt) {
+          const int64_t from = s_from[k];
+          if (from >= 0)
+            nx[i] = *reinterpret_cast<const U *>(pool + from + off);
+        }
+      }
+    };
+    fetch(0);
+    for (uint32_t k0 = 0; k0 < cnt; k0 += round) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        x[i] = nx[i];
+      if (k0 + round < cnt)
+        fetch(k0 + round);
+      // this round's rows are in registers on every lane before any of them is written: each
+      // lane waits for its own here (the next round's stay under way), then the barrier
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        hold(x[i]);
+      asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t k = k0 + (uint32_t)i * rows + rr;
+        if (active && k < cnt && s_from[k] >= 0) {
+          if constexpr (FP8) {
+            const float inv = s_inv[k];
+            if (inv != 0.f) {
+              const float was = s_old[k];
+              uint8_t *b = reinterpret_cast<uint8_t *>(&x[i]);
+#pragma unroll
+              for (uint32_t c = 0; c < sizeof(U); ++c)
+                b[c] = (uint8_t)recode(b[c], was, inv);
+            }
+          }
+          *reinterpret_cast<U *>(pool + s_to[k] + off) = x[i];
+        }
+      }
+    }
+  }
+}
+
+// fp8: the new scales, once no move reads the old ones.
+__global__ void __launch_bounds__(256) evict_scales(EParams P) {
+  const uint32_t task = blockIdx.x, r = task / P.Hkv, h = task % P.Hkv;
+  const Req q = req_of(P, r);
+  if (q.m == q.n || q.m == 0u || P.kept[(int64_t)task * P.max_keep] < 0)
+    return;
+  const float *ns = P.new_scale + (int64_t)task * 2 * P.new_pages;
+  for (uint32_t b = threadIdx.x; b * P.ps < q.m; b += 256u) {
+    const int64_t si = ((int64_t)P.bt[q.row + b] * P.Hkv + h) * P.scale_stride;
+    P.ks[si] = ns[b];
+    P.vs[si] = ns[P.new_pages + b];
   }
 }
 
@@ -299,10 +508,16 @@ int check_shape(const SchedEvictArgs *a) {
     return set_error(-1, "sched_kv_evict: page_size %u (multiple of 4, <= 256)", a->page_size);
   if (a->num_pages == 0 || a->num_pages > 0x7fffffffull)
     return set_error(-1, "sched_kv_evict: num_pages %llu", (unsigned long long)a->num_pages);
+  if ((uint64_t)a->max_pages * a->page_size > (1u << 24))
+    return set_error(-1, "sched_kv_evict: tables of %u pages of %u tokens (at most 2^24 tokens)",
+                     a->max_pages, a->page_size);
   if (a->max_keep > 0x7fffffffu)
     return set_error(-1, "sched_kv_evict: max_keep %u", a->max_keep);
   return 0;
 }
+
+// Workgroups of the move that fill the card.
+constexpr uint32_t kMoveFill = 512;
 
 uint32_t new_pages_of(const SchedEvictArgs *a) {
   return (uint32_t)(((uint64_t)a->max_keep + a->page_size - 1u) / a->page_size);
@@ -370,9 +585,15 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   P.new_pages = new_pages_of(a);
   P.sink = a->sink, P.recent = a->recent, P.num_pages = (uint32_t)a->num_pages;
 
+  P.ps_magic = 0xffffffffu / P.ps + 1u;
+
   const uint32_t tasks = P.R * P.Hkv;
+  const uint64_t longest = (uint64_t)a->max_pages * a->page_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  hipLaunchKernelGGL(evict_select, dim3(tasks), dim3(kSelect), 0, s, P);
+  if (longest <= 256u * 16u)
+    hipLaunchKernelGGL((evict_select<256, 16>), dim3(tasks), dim3(256), 0, s, P);
+  else
+    hipLaunchKernelGGL((evict_select<1024, 32>), dim3(tasks), dim3(1024), 0, s, P);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a->max_keep > 0) {
     auto rows16 = [&](int64_t x) { return (x * eb) % 16 == 0; };
@@ -382,18 +603,27 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
                       rows16(P.vhs) && rows16(P.vts);
     const uint32_t units = wide ? a->head_dim * eb / 16u : a->head_dim;
     const int64_t k_step = wide ? 16 : eb, v_step = wide ? 16 : a->v_dim_stride * eb;
-    const dim3 grid(2u * tasks), block(kMove);
+    // few tasks: a row in up to four parts, of 64 bytes at least, for more workgroups
+    uint32_t parts = 1;
+    while (wide && parts < 4u && 2u * tasks * parts < kMoveFill && units / (2u * parts) >= 4u)
+      parts *= 2u;
+    const uint32_t part = (units + parts - 1u) / parts;
+    const dim3 grid(2u * tasks * parts), block(kMove);
     if (wide && fp8)
-      hipLaunchKernelGGL((evict_move<uint4, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint4, true>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
     else if (wide)
-      hipLaunchKernelGGL((evict_move<uint4, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint4, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
     else if (fp8)
-      hipLaunchKernelGGL((evict_move<uint8_t, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint8_t, true>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
     else if (eb == 2)
-      hipLaunchKernelGGL((evict_move<uint16_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint16_t, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
     else
-      hipLaunchKernelGGL((evict_move<uint32_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint32_t, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
     e = hipGetLastError();
+    if (e == hipSuccess && fp8) {
+      hipLaunchKernelGGL(evict_scales, dim3(tasks), dim3(256), 0, s, P);
+      e = hipGetLastError();
+    }
   }
   if (e != hipSuccess)
     return set_error(-1, "sched_kv_evict: launch failed: %s", hipGetErrorString(e));

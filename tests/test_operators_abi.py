@@ -135,6 +135,7 @@ def evict_args(**kw):
     (dict(num_kv_heads=0), "kv-heads"), (dict(head_dim=0), "head_dim"),
     (dict(head_dim=260), "head_dim"), (dict(page_size=6), "page_size"),
     (dict(num_pages=0), "num_pages"), (dict(max_keep=1 << 31), "max_keep"),
+    (dict(max_pages=1 << 21, bt_stride=1 << 21), "2^24 tokens"),
     (dict(weights=None), "required"), (dict(kept=None), "required"), (dict(bt_stride=3), "bt_stride"),
     (dict(v_dim_stride=2), "V needs"), (dict(k_pool=ctypes.c_void_p(0x10001)), "aligned"),
     (dict(kv_dtype=abi.FP8_E4M3), "k_scale"),
