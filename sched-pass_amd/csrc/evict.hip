@@ -6,7 +6,7 @@
 //           like it, eight at a time from the highest that differ: a histogram, then the
 //           digit in which the wanted rank falls), then keeps, in order, those above T
 //           and the first ties. Its keys stay in registers, each weight is read once.
-//   move:   one workgroup per (request, kv-head, keys or values, part of the row) copies
+//   move:   one workgroup per (request, kv-head, keys or values) copies
 //           the kept rows down, a round of rows at a time. A row's new slot is never
 //           behind its old one, so what a round overwrites are rows of its own or of
 //           earlier rounds: it may be written once all of it has been read, with the next
@@ -41,6 +41,12 @@ struct EParams {
   uint32_t sink, recent;
   uint32_t num_pages;
   uint32_t ps_magic; // ceil(2^32 / ps): t / ps for t up to 2^24
+  uint32_t row_groups; // evict_move: workgroups that move rows (then weights, a task each)
+  // the wide selection: per task three histograms, whether its table is bad, and per chunk
+  // its kept tokens and ties
+  uint32_t *wide, chunks;
+  // evict_move_few: per task and tensor a ticket and a flag for each of its chunks
+  uint32_t *moves, move_chunks;
 };
 
 struct Req {
@@ -97,9 +103,23 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t x, uint32_t *s_wave, uin
   return x + before;
 }
 
+// evict_move_few's tickets and flags of a task's keys and values, none taken or set.
+__device__ __forceinline__ void clear_moves(const EParams &P, uint32_t task, uint32_t nt) {
+  if (P.moves == nullptr)
+    return;
+  const uint32_t each = 1u + P.move_chunks;
+  for (uint32_t k = threadIdx.x; k < 2u * each; k += nt)
+    P.moves[(uint64_t)task * 2u * each + k] = 0u;
+}
+
+// Histograms come in kCopies, a lane's by its number: weights share their exponents, and
+// one counter serves one lane at a time.
+constexpr uint32_t kCopies = 8;
+
 // The digit of s_hist (256 counts) in which the left-th largest falls, and how many lie
 // above it; by the first wave, four digits a lane.
-__device__ __forceinline__ void pick_digit(const uint32_t *s_hist, uint32_t left, uint32_t *s_pick) {
+__device__ __forceinline__ void pick_digit(const uint32_t (*s_hist)[256], uint32_t left,
+                                           uint32_t *s_pick) {
   const uint32_t lane = threadIdx.x;
   if (lane >= 64u)
     return;
@@ -107,7 +127,10 @@ __device__ __forceinline__ void pick_digit(const uint32_t *s_hist, uint32_t left
   uint32_t c[4], sum = 0u;
 #pragma unroll
   for (uint32_t k = 0; k < 4; ++k) {
-    c[k] = s_hist[255u - (4u * lane + k)];
+    c[k] = 0u;
+#pragma unroll
+    for (uint32_t p = 0; p < kCopies; ++p)
+      c[k] += s_hist[p][255u - (4u * lane + k)];
     sum += c[k];
   }
   uint32_t incl = sum;
@@ -130,13 +153,140 @@ __device__ __forceinline__ void pick_digit(const uint32_t *s_hist, uint32_t left
   }
 }
 
+// The kept tokens of a stretch in order: NT lanes with KREG tokens each, x their weights (token
+// t0 + i NT + lane). Those outside [lo, hi) stay, of the others those whose key is above T
+// and the first `left` of key T; *base and *seen are the kept tokens and the ties before
+// the stretch, and go on. WEIGHTS: their weights move along (in place: every lane has the
+// stretch's before one is overwritten, and those of later stretches lie behind every slot
+// that is written here).
+template <int NT, int KREG, bool WEIGHTS>
+__device__ __forceinline__ void keep_stretch(const EParams &P, const Req &q, uint32_t h,
+                                             const float (&x)[KREG], uint32_t t0, uint32_t lo,
+                                             uint32_t hi, uint32_t want, uint32_t T,
+                                             uint32_t left, int32_t *kept, uint32_t *s_cnt,
+                                             uint32_t *s_wave, uint32_t *base, uint32_t *seen) {
+  constexpr uint32_t NW = NT / 64;
+  constexpr uint32_t E = (KREG * NW + NT - 1) / NT; // counts of a lane in a scan
+  static_assert(KREG <= 32, "a bit for each token of a lane");
+  const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+  const bool cut = q.m < q.n;
+  const unsigned long long below = (1ull << lane) - 1ull;
+  // exclusive sums, in token order, of the counts per (i, wave); returns their sum
+  auto scan = [&]() __attribute__((always_inline)) {
+    __syncthreads();
+    uint32_t c[E], sum = 0u, all;
+#pragma unroll
+    for (uint32_t k = 0; k < E; ++k) {
+      const uint32_t e = tid * E + k;
+      c[k] = e < KREG * NW && t0 + e / NW * NT < q.n ? s_cnt[e] : 0u;
+      sum += c[k];
+    }
+    uint32_t at = block_scan<NT>(sum, s_wave, &all) - sum;
+#pragma unroll
+    for (uint32_t k = 0; k < E; ++k) {
+      const uint32_t e = tid * E + k;
+      if (e < KREG * NW)
+        s_cnt[e] = at;
+      at += c[k];
+    }
+    __syncthreads();
+    return all;
+  };
+  uint32_t stay = 0u; // bit i: this lane's token i is kept
+  if (cut && left > 0u) {
+#pragma unroll
+    for (int i = 0; i < KREG; ++i) {
+      if (t0 + (uint32_t)i * NT >= q.n)
+        break;
+      const uint32_t t = t0 + (uint32_t)i * NT + tid;
+      const unsigned long long b = __ballot(t >= lo && t < hi && order_bits(x[i]) == T);
+      if (lane == 0)
+        s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
+    }
+    const uint32_t all = scan();
+#pragma unroll
+    for (int i = 0; i < KREG; ++i) {
+      if (t0 + (uint32_t)i * NT >= q.n)
+        break;
+      const uint32_t t = t0 + (uint32_t)i * NT + tid;
+      const bool tie = t >= lo && t < hi && order_bits(x[i]) == T;
+      const unsigned long long b = __ballot(tie);
+      if (tie && *seen + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below) < left)
+        stay |= 1u << i;
+    }
+    *seen += all;
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < KREG; ++i) {
+    if (t0 + (uint32_t)i * NT >= q.n)
+      break;
+    const uint32_t t = t0 + (uint32_t)i * NT + tid;
+    if (t < q.n && (!cut || t < lo || t >= hi || (want > 0u && order_bits(x[i]) > T)))
+      stay |= 1u << i;
+    const unsigned long long b = __ballot((stay >> i) & 1u);
+    if (lane == 0)
+      s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
+  }
+  __builtin_amdgcn_s_waitcnt(kVmcnt0);
+  const uint32_t all = scan();
+#pragma unroll
+  for (int i = 0; i < KREG; ++i) {
+    if (t0 + (uint32_t)i * NT >= q.n)
+      break;
+    const uint32_t t = t0 + (uint32_t)i * NT + tid;
+    const bool in = (stay >> i) & 1u;
+    const unsigned long long b = __ballot(in);
+    const uint32_t at = *base + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below);
+    if (in && at < q.m) {
+      kept[at] = (int32_t)t;
+      if (WEIGHTS && (t != at || P.wo != P.w)) {
+        const uint32_t d = div_ps(P, at);
+        P.wo[(int64_t)P.bt[q.row + d] * P.w_ps + (int64_t)h * P.w_hs + (at - d * P.ps)] = x[i];
+      }
+    }
+  }
+  *base += all;
+  __syncthreads();
+}
+
+// fp8: the new scales of the pages that will hold a task's kept tokens (`kept` written and
+// visible), whole pages of up to NT tokens at a time, from round y on, every ny-th: a
+// page's is the largest of its tokens' old ones (scales are not negative: their bits
+// order like them).
+template <int NT>
+__device__ __forceinline__ void new_scales(const EParams &P, const Req &q, uint32_t task, uint32_t h,
+                                           const int32_t *kept, uint32_t y, uint32_t ny) {
+  __shared__ uint32_t s_max[2][NT / 4];
+  float *ns = P.new_scale + (int64_t)task * 2 * P.new_pages;
+  const uint32_t pages = NT / P.ps, span = pages * P.ps; // (ps is 4 to 256, NT 256 or more)
+  for (uint32_t j0 = y * span; j0 < q.m; j0 += ny * span) {
+    for (uint32_t b = threadIdx.x; b < pages; b += NT)
+      s_max[0][b] = s_max[1][b] = 0u;
+    __syncthreads();
+    const uint32_t j = j0 + threadIdx.x;
+    if (threadIdx.x < span && j < q.m) {
+      const int64_t si =
+          ((int64_t)P.bt[q.row + div_ps(P, (uint32_t)kept[j])] * P.Hkv + h) * P.scale_stride;
+      const uint32_t b = div_ps(P, threadIdx.x);
+      atomicMax(&s_max[0][b], __float_as_uint(fmaxf(P.ks[si], 0.f)));
+      atomicMax(&s_max[1][b], __float_as_uint(fmaxf(P.vs[si], 0.f)));
+    }
+    __syncthreads();
+    for (uint32_t b = threadIdx.x; b < pages && j0 + b * P.ps < q.m; b += NT) {
+      ns[j0 / P.ps + b] = __uint_as_float(s_max[0][b]);
+      ns[P.new_pages + j0 / P.ps + b] = __uint_as_float(s_max[1][b]);
+    }
+    __syncthreads();
+  }
+}
+
 // NT lanes with KREG tokens each in registers, a stretch (its token t0 + i NT + lane). A
 // request of one stretch is read once; a longer one stretch by stretch for each digit.
 template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(EParams P) {
+  clear_moves(P, blockIdx.x, NT);
   constexpr uint32_t NW = NT / 64, SPAN = NT * KREG;
-  constexpr uint32_t E = (KREG * NW + NT - 1) / NT; // counts of a lane in a scan
-  static_assert(KREG <= 32, "a bit for each token of a lane");
-  __shared__ uint32_t s_hist[256];
+  __shared__ uint32_t s_hist[kCopies][256];
   __shared__ uint32_t s_cnt[KREG * NW];
   __shared__ uint32_t s_wave[NW], s_pick[3], s_lo[NW], s_hi[NW];
   __shared__ uint32_t s_bad;
@@ -176,6 +326,8 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
         const uint32_t b = div_ps(P, t);
         x[i] = w0[(int64_t)P.bt[q.row + b] * P.w_ps + (t - b * P.ps)];
       }
+      if (i % 8 == 7) // eight tokens' addresses at a time
+        __builtin_amdgcn_sched_barrier(0);
     }
   };
   load(0);
@@ -218,8 +370,8 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
     while (top > 0) {
       const int shift = top > 8 ? top - 8 : 0;
       const uint32_t mask = (1u << (top - shift)) - 1u; // a digit of at most eight bits
-      for (uint32_t k = tid; k < 256u; k += NT)
-        s_hist[k] = 0u;
+      for (uint32_t k = tid; k < kCopies * 256u; k += NT)
+        (&s_hist[0][0])[k] = 0u;
       __syncthreads();
       for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
         if (!one)
@@ -231,7 +383,7 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
           const uint32_t t = t0 + (uint32_t)i * NT + tid;
           const uint32_t key = order_bits(x[i]);
           if (t >= lo && t < hi && (top >= 32 || (key >> top) == (T >> top)))
-            atomicAdd(&s_hist[(key >> shift) & mask], 1u);
+            atomicAdd(&s_hist[lane % kCopies][(key >> shift) & mask], 1u);
         }
       }
       __syncthreads();
@@ -250,111 +402,211 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
     }
   }
 
-  // exclusive sums, in token order, of the stretch's counts per (i, wave); returns their sum
-  auto scan = [&](uint32_t t0) __attribute__((always_inline)) {
-    __syncthreads();
-    uint32_t c[E], sum = 0u, all;
-#pragma unroll
-    for (uint32_t k = 0; k < E; ++k) {
-      const uint32_t e = tid * E + k;
-      c[k] = e < KREG * NW && t0 + e / NW * NT < q.n ? s_cnt[e] : 0u;
-      sum += c[k];
-    }
-    uint32_t at = block_scan<NT>(sum, s_wave, &all) - sum;
-#pragma unroll
-    for (uint32_t k = 0; k < E; ++k) {
-      const uint32_t e = tid * E + k;
-      if (e < KREG * NW)
-        s_cnt[e] = at;
-      at += c[k];
-    }
-    __syncthreads();
-    return all;
-  };
   uint32_t base = 0u, seen = 0u; // kept tokens and ties of the stretches before
-  const unsigned long long below = (1ull << lane) - 1ull;
   for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
     if (!one)
       load(t0);
-    uint32_t stay = 0u; // bit i: this lane's token i is kept
-    if (cut && left > 0u) { // the first `left` tokens of weight T are
-#pragma unroll
-      for (int i = 0; i < KREG; ++i) {
-        if (t0 + (uint32_t)i * NT >= q.n)
-          break;
-        const uint32_t t = t0 + (uint32_t)i * NT + tid;
-        const unsigned long long b = __ballot(t >= lo && t < hi && order_bits(x[i]) == T);
-        if (lane == 0)
-          s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
-      }
-      const uint32_t all = scan(t0);
-#pragma unroll
-      for (int i = 0; i < KREG; ++i) {
-        if (t0 + (uint32_t)i * NT >= q.n)
-          break;
-        const uint32_t t = t0 + (uint32_t)i * NT + tid;
-        const bool tie = t >= lo && t < hi && order_bits(x[i]) == T;
-        const unsigned long long b = __ballot(tie);
-        if (tie && seen + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below) < left)
-          stay |= 1u << i;
-      }
-      seen += all;
-      __syncthreads();
-    }
-#pragma unroll
-    for (int i = 0; i < KREG; ++i) {
-      if (t0 + (uint32_t)i * NT >= q.n)
-        break;
-      const uint32_t t = t0 + (uint32_t)i * NT + tid;
-      if (t < q.n && (!cut || t < lo || t >= hi || (want > 0u && order_bits(x[i]) > T)))
-        stay |= 1u << i;
-      const unsigned long long b = __ballot((stay >> i) & 1u);
-      if (lane == 0)
-        s_cnt[i * NW + wave] = (uint32_t)__popcll(b);
-    }
-    // in place: every lane has this stretch's weights before one is overwritten; those of
-    // later stretches lie behind every slot that is written now
-    __builtin_amdgcn_s_waitcnt(kVmcnt0);
-    const uint32_t all = scan(t0);
-#pragma unroll
-    for (int i = 0; i < KREG; ++i) {
-      if (t0 + (uint32_t)i * NT >= q.n)
-        break;
-      const uint32_t t = t0 + (uint32_t)i * NT + tid;
-      const bool in = (stay >> i) & 1u;
-      const unsigned long long b = __ballot(in);
-      const uint32_t at = base + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below);
-      if (in && at < q.m) {
-        kept[at] = (int32_t)t;
-        if (t != at || P.wo != P.w) {
-          const uint32_t d = div_ps(P, at);
-          P.wo[(int64_t)P.bt[q.row + d] * P.w_ps + (int64_t)h * P.w_hs + (at - d * P.ps)] = x[i];
-        }
-      }
-    }
-    base += all;
-    __syncthreads();
+    keep_stretch<NT, KREG, true>(P, q, h, x, t0, lo, hi, want, T, left, kept, s_cnt, s_wave, &base,
+                                 &seen);
   }
   for (uint32_t j = q.m + tid; j < P.max_keep; j += NT)
     kept[j] = -1;
-  // fp8: the new scales of the pages that hold the kept tokens
   if (P.new_scale != nullptr && cut) {
     __builtin_amdgcn_s_waitcnt(kVmcnt0);
     __syncthreads();
-    float *ns = P.new_scale + (int64_t)task * 2 * P.new_pages;
-    for (uint32_t b = tid; b * P.ps < q.m; b += NT) {
-      float mk = 0.f, mv = 0.f;
-      const uint32_t end = min(q.m, (b + 1u) * P.ps);
-      for (uint32_t j = b * P.ps; j < end; ++j) {
-        const int64_t si =
-            ((int64_t)P.bt[q.row + div_ps(P, (uint32_t)kept[j])] * P.Hkv + h) * P.scale_stride;
-        mk = fmaxf(mk, P.ks[si]);
-        mv = fmaxf(mv, P.vs[si]);
+    new_scales<NT>(P, q, task, h, kept, 0u, 1u);
+  }
+}
+
+// ---- few long requests: a task's tokens over many workgroups ----------------------
+// The same selection in steps: wide_start checks the table and clears the histograms; three
+// wide_digit launches count the digits [31:21], [20:10] and [9:0] of the keys, each among those
+// that agree with the digits before; wide_count counts each chunk's kept tokens and ties;
+// wide_keep writes them. Weights move with the rows, in evict_move's grid.
+constexpr int kWide = 256, kWideReg = 16;
+constexpr uint32_t kWideSpan = kWide * kWideReg, kWideBins = 2048;
+
+__device__ __forceinline__ uint32_t *wide_hist(const EParams &P, uint32_t task) {
+  return P.wide + (uint64_t)task * (3u * kWideBins + 1u + 2u * P.chunks);
+}
+
+// What a task's tokens compete for; false: the request is not cut, or has a bad table.
+struct Contest {
+  Req q;
+  uint32_t task, r, h, lo, hi, want;
+};
+__device__ __forceinline__ Contest contest_of(const EParams &P) {
+  Contest c;
+  c.task = blockIdx.x, c.r = c.task / P.Hkv, c.h = c.task % P.Hkv;
+  c.q = req_of(P, c.r);
+  const uint32_t recent = min(c.q.m, P.recent);
+  c.lo = min(P.sink, c.q.m - recent);
+  c.hi = c.q.n - recent;
+  c.want = c.q.m - recent - c.lo;
+  return c;
+}
+
+__global__ void __launch_bounds__(kWide) wide_start(EParams P) {
+  __shared__ uint32_t s_bad;
+  const Contest c = contest_of(P);
+  uint32_t *hist = wide_hist(P, c.task);
+  clear_moves(P, c.task, kWide);
+  if (threadIdx.x == 0)
+    s_bad = c.q.ok ? 0u : 1u;
+  __syncthreads();
+  if (c.q.ok)
+    for (uint32_t b = threadIdx.x; b * (uint64_t)P.ps < c.q.n; b += kWide)
+      if ((uint32_t)P.bt[c.q.row + b] >= P.num_pages)
+        s_bad = 1u;
+  for (uint32_t k = threadIdx.x; k < 3u * kWideBins; k += kWide)
+    hist[k] = 0u;
+  __syncthreads();
+  const uint32_t bad = s_bad;
+  if (threadIdx.x == 0) {
+    hist[3u * kWideBins] = bad;
+    if (bad && P.errors)
+      atomicAdd(P.errors, 1u);
+  }
+  int32_t *kept = P.kept + (int64_t)c.task * P.max_keep;
+  for (uint32_t j = (bad ? 0u : c.q.m) + threadIdx.x; j < P.max_keep; j += kWide)
+    kept[j] = -1;
+}
+
+// The key prefix of the last kept token after `digits` digits, and how many of the tokens that
+// share it are kept.
+__device__ __forceinline__ void wide_pick(const uint32_t *hist, int digits, uint32_t want,
+                                          uint32_t *s_wave, uint32_t *s_pick, uint32_t *T,
+                                          uint32_t *left) {
+  constexpr uint32_t PER = kWideBins / kWide;
+  *T = 0u, *left = want;
+  for (int p = 0; p < digits; ++p) {
+    uint32_t c[PER], sum = 0u, all;
+#pragma unroll
+    for (uint32_t k = 0; k < PER; ++k) { // lane 0 has the highest digits
+      c[k] = hist[p * kWideBins + kWideBins - 1u - (threadIdx.x * PER + k)];
+      sum += c[k];
+    }
+    uint32_t above = block_scan<kWide>(sum, s_wave, &all) - sum;
+#pragma unroll
+    for (uint32_t k = 0; k < PER; ++k) {
+      if (above < *left && *left <= above + c[k]) {
+        s_pick[0] = kWideBins - 1u - (threadIdx.x * PER + k);
+        s_pick[1] = above;
       }
-      ns[b] = mk;
-      ns[P.new_pages + b] = mv;
+      above += c[k];
+    }
+    __syncthreads();
+    *T |= s_pick[0] << (p == 0 ? 21 : p == 1 ? 10 : 0);
+    *left -= s_pick[1];
+    __syncthreads();
+  }
+}
+
+__device__ __forceinline__ void wide_load(const EParams &P, const Contest &c, uint32_t t0,
+                                          float (&x)[kWideReg]) {
+  const float *w0 = P.w + (int64_t)c.h * P.w_hs;
+#pragma unroll
+  for (int i = 0; i < kWideReg; ++i) {
+    const uint32_t t = t0 + (uint32_t)i * kWide + threadIdx.x;
+    x[i] = 0.f;
+    if (t < c.q.n) {
+      const uint32_t b = div_ps(P, t);
+      x[i] = w0[(int64_t)P.bt[c.q.row + b] * P.w_ps + (t - b * P.ps)];
     }
   }
+}
+
+__global__ void __launch_bounds__(kWide) wide_digit(EParams P, int digit) {
+  __shared__ uint32_t s_hist[kWideBins], s_wave[kWide / 64], s_pick[2];
+  const Contest c = contest_of(P);
+  uint32_t *hist = wide_hist(P, c.task);
+  const uint32_t t0 = blockIdx.y * kWideSpan;
+  if (t0 >= c.q.n || c.q.m == c.q.n || c.want == 0u || hist[3u * kWideBins])
+    return;
+  float x[kWideReg];
+  wide_load(P, c, t0, x);
+  for (uint32_t k = threadIdx.x; k < kWideBins; k += kWide)
+    s_hist[k] = 0u;
+  uint32_t T, left;
+  wide_pick(hist, digit, c.want, s_wave, s_pick, &T, &left);
+  __syncthreads();
+  const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, top = digit == 1 ? 21 : 10;
+  const uint32_t mask = digit == 2 ? 1023u : 2047u;
+#pragma unroll
+  for (int i = 0; i < kWideReg; ++i) {
+    const uint32_t t = t0 + (uint32_t)i * kWide + threadIdx.x, key = order_bits(x[i]);
+    if (t >= c.lo && t < c.hi && (digit == 0 || (key >> top) == (T >> top)))
+      atomicAdd(&s_hist[(key >> shift) & mask], 1u);
+  }
+  __syncthreads();
+  for (uint32_t k = threadIdx.x; k < kWideBins; k += kWide)
+    if (s_hist[k])
+      atomicAdd(&hist[digit * kWideBins + k], s_hist[k]);
+}
+
+__global__ void __launch_bounds__(kWide) wide_count(EParams P) {
+  __shared__ uint32_t s_wave[kWide / 64], s_pick[2];
+  const Contest c = contest_of(P);
+  uint32_t *hist = wide_hist(P, c.task), *cnt = hist + 3u * kWideBins + 1u;
+  const uint32_t t0 = blockIdx.y * kWideSpan;
+  if (t0 >= c.q.n || c.q.m == c.q.n || hist[3u * kWideBins])
+    return;
+  float x[kWideReg];
+  wide_load(P, c, t0, x);
+  uint32_t T = 0u, left = 0u;
+  if (c.want > 0u)
+    wide_pick(hist, 3, c.want, s_wave, s_pick, &T, &left);
+  uint32_t stay = 0u, ties = 0u, all;
+#pragma unroll
+  for (int i = 0; i < kWideReg; ++i) {
+    const uint32_t t = t0 + (uint32_t)i * kWide + threadIdx.x, key = order_bits(x[i]);
+    const bool mid = t >= c.lo && t < c.hi;
+    stay += t < c.q.n && (!mid || (c.want > 0u && key > T));
+    ties += mid && c.want > 0u && key == T;
+  }
+  block_scan<kWide>(stay, s_wave, &all);
+  if (threadIdx.x == 0)
+    cnt[2u * blockIdx.y] = all;
+  block_scan<kWide>(ties, s_wave, &all);
+  if (threadIdx.x == 0)
+    cnt[2u * blockIdx.y + 1u] = all;
+}
+
+__global__ void __launch_bounds__(kWide) wide_keep(EParams P) {
+  __shared__ uint32_t s_cnt[kWideReg * (kWide / 64)], s_wave[kWide / 64], s_pick[2];
+  const Contest c = contest_of(P);
+  uint32_t *hist = wide_hist(P, c.task), *cnt = hist + 3u * kWideBins + 1u;
+  const uint32_t t0 = blockIdx.y * kWideSpan;
+  if (t0 >= c.q.n || hist[3u * kWideBins])
+    return;
+  const bool cut = c.q.m < c.q.n;
+  float x[kWideReg];
+  wide_load(P, c, t0, x);
+  uint32_t T = 0u, left = 0u, base = 0u, seen = 0u;
+  if (cut) {
+    if (c.want > 0u)
+      wide_pick(hist, 3, c.want, s_wave, s_pick, &T, &left);
+    uint32_t a = 0u, b = 0u;
+    for (uint32_t k = threadIdx.x; k < blockIdx.y; k += kWide) {
+      a += cnt[2u * k];
+      b += cnt[2u * k + 1u];
+    }
+    block_scan<kWide>(a, s_wave, &base);
+    block_scan<kWide>(b, s_wave, &seen);
+    base += min(seen, left);
+  } else {
+    base = t0;
+  }
+  keep_stretch<kWide, kWideReg, false>(P, c.q, c.h, x, t0, c.lo, c.hi, c.want, T, left,
+                                       P.kept + (int64_t)c.task * P.max_keep, s_cnt, s_wave, &base,
+                                       &seen);
+}
+
+__global__ void __launch_bounds__(1024) wide_scales(EParams P) {
+  const Contest c = contest_of(P);
+  const int32_t *kept = P.kept + (int64_t)c.task * P.max_keep;
+  if (c.q.m < c.q.n && c.q.m > 0u && kept[0] >= 0)
+    new_scales<1024>(P, c.q, c.task, c.h, kept, blockIdx.y, gridDim.y);
 }
 
 // Makes the compiler wait for a load into x here.
@@ -369,29 +621,76 @@ __device__ __forceinline__ void hold(uint8_t &x) {
   x = (uint8_t)y;
 }
 
-// One e4m3 code from a page of scale s in a page of scale `to` (inv = 1 / to).
-__device__ __forceinline__ uint32_t recode(uint32_t c, float s, float inv) {
-  if ((c & 0x7fu) == 0x7fu)
-    return c;
-  const float x = fp8e4m3_to_f32(c) * s * inv;
-  return encode2_fp8(x, 0.f) & 0xffu;
+// Four e4m3 codes times f, encoded anew; NaN codes as they are.
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float f) {
+  typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+  const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const f32x2_t b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  const float q[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
+  uint32_t y = encode4_fp8(q);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t m = 0x7fu << (8 * k), all = 0xffu << (8 * k);
+    y = (c & m) == m ? (y & ~all) | (c & all) : y;
+  }
+  return y;
 }
+__device__ __forceinline__ void recode(uint4 &x, float f) {
+  x.x = recode4(x.x, f), x.y = recode4(x.y, f), x.z = recode4(x.z, f), x.w = recode4(x.w, f);
+}
+__device__ __forceinline__ void recode(uint8_t &x, float f) { x = (uint8_t)recode4(x, f); }
+template <typename U> __device__ __forceinline__ void recode(U &, float) {}
 
 constexpr int kMove = 512;
 constexpr uint32_t kStage = 2048; // rows whose places are in LDS at a time
 
+// A task's weights after the wide selection, by one workgroup: as the rows below, a round of
+// kMove * 8 weights read before it is written.
+__device__ __forceinline__ void move_weights(const EParams &P, uint32_t task) {
+  constexpr int N = 8;
+  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
+  const Req q = req_of(P, r);
+  const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
+  if (q.m == 0u || kept[0] < 0 || (q.m == q.n && P.wo == P.w))
+    return;
+  for (uint32_t j0 = 0; j0 < q.m; j0 += kMove * N) {
+    float x[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t j = j0 + (uint32_t)i * kMove + threadIdx.x;
+      if (j < q.m) {
+        const uint32_t t = (uint32_t)kept[j], b = div_ps(P, t);
+        x[i] = P.w[(int64_t)P.bt[q.row + b] * P.w_ps + (int64_t)h * P.w_hs + (t - b * P.ps)];
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(kVmcnt0);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t j = j0 + (uint32_t)i * kMove + threadIdx.x;
+      if (j < q.m) {
+        const uint32_t b = div_ps(P, j);
+        P.wo[(int64_t)P.bt[q.row + b] * P.w_ps + (int64_t)h * P.w_hs + (j - b * P.ps)] = x[i];
+      }
+    }
+  }
+}
+
 // U: the unit a row is moved in (16 bytes where rows are contiguous and aligned, else
-// one element); a row is `units` of them, k_step / v_step bytes apart, `part` of them this
-// workgroup's.
+// one element); a row is `units` of them, k_step / v_step bytes apart.
 template <typename U, bool FP8>
-__global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, uint32_t part,
+__global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units,
                                                     int64_t k_step, int64_t v_step, uint32_t eb) {
   constexpr int N = 4; // units of a lane and round
-  // where a row comes from (-1: it stays) and goes to; fp8: its old scale, the new one's inverse
+  // where a row comes from (-1: it stays) and goes to; fp8: its old scale over the new one
   __shared__ int64_t s_from[kStage], s_to[kStage];
-  __shared__ float s_old[FP8 ? kStage : 1], s_inv[FP8 ? kStage : 1];
-  const uint32_t tid = threadIdx.x, tasks2 = 2u * P.R * P.Hkv;
-  const uint32_t which = blockIdx.x % tasks2, first = blockIdx.x / tasks2 * part;
+  __shared__ float s_ratio[FP8 ? kStage : 1];
+  const uint32_t tid = threadIdx.x;
+  if (blockIdx.x >= P.row_groups) { // the wide selection's weights
+    move_weights(P, blockIdx.x - P.row_groups);
+    return;
+  }
+  const uint32_t which = blockIdx.x;
   const uint32_t task = which >> 1;
   const bool vals = (which & 1u) != 0u;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
@@ -403,8 +702,8 @@ __global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, u
   const int64_t ps_b = (vals ? P.vps : P.kps) * eb, ts_b = (vals ? P.vts : P.kts) * eb;
   const float *scale = vals ? P.vs : P.ks;
   const float *ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
-  const uint32_t e = first + tid % part, rr = tid / part, rows = kMove / part;
-  const bool active = rr < rows && e < units;
+  const uint32_t e = tid % units, rr = tid / units, rows = kMove / units;
+  const bool active = rr < rows;
   const int64_t off = (int64_t)e * (vals ? v_step : k_step);
   const uint32_t round = rows * N;
 
@@ -418,8 +717,7 @@ __global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, u
       bool moves = src != j;
       if constexpr (FP8) {
         const float was = scale[(sp * P.Hkv + h) * P.scale_stride], now = ns[db];
-        s_old[i] = was;
-        s_inv[i] = was != now ? 1.f / now : 0.f; // 0: the codes stay
+        s_ratio[i] = was != now ? was / now : -1.f; // below 0: the codes stay
         moves = moves || was != now;
       }
       s_from[i] = moves ? sp * ps_b + (int64_t)(src - sb * P.ps) * ts_b : -1;
@@ -457,18 +755,98 @@ __global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units, u
         const uint32_t k = k0 + (uint32_t)i * rows + rr;
         if (active && k < cnt && s_from[k] >= 0) {
           if constexpr (FP8) {
-            const float inv = s_inv[k];
-            if (inv != 0.f) {
-              const float was = s_old[k];
-              uint8_t *b = reinterpret_cast<uint8_t *>(&x[i]);
-#pragma unroll
-              for (uint32_t c = 0; c < sizeof(U); ++c)
-                b[c] = (uint8_t)recode(b[c], was, inv);
-            }
+            const float f = s_ratio[k];
+            if (f >= 0.f)
+              recode(x[i], f);
           }
           *reinterpret_cast<U *>(pool + s_to[k] + off) = x[i];
         }
       }
+    }
+  }
+}
+
+// Few tasks: a task's rows over many workgroups. Each takes the next chunk of its (task, keys
+// or values) by a ticket, reads the chunk's rows into registers, says so, and writes them once
+// all chunks before it have said so: what it overwrites are rows of theirs or its own. A
+// chunk waits for earlier tickets only, whose workgroups are running and wait for nothing
+// before they say so; every wait ends.
+constexpr int kFewUnits = 8; // units of a lane
+
+template <bool FP8>
+__global__ void __launch_bounds__(kMove) evict_move_few(EParams P, uint32_t units, uint32_t eb) {
+  constexpr uint32_t MOST = kMove / 4 * kFewUnits; // rows of a chunk (4 units a row at least)
+  __shared__ int64_t s_from[MOST], s_to[MOST];
+  __shared__ float s_ratio[FP8 ? MOST : 1];
+  __shared__ uint32_t s_chunk;
+  if (blockIdx.x >= P.row_groups) { // the wide selection's weights
+    move_weights(P, blockIdx.x - P.row_groups);
+    return;
+  }
+  const uint32_t tid = threadIdx.x, which = blockIdx.x % (2u * P.R * P.Hkv), task = which >> 1;
+  const bool vals = (which & 1u) != 0u;
+  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
+  const Req q = req_of(P, r);
+  const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
+  if (q.m == q.n || q.m == 0u || kept[0] < 0)
+    return;
+  uint32_t *ticket = P.moves + (uint64_t)which * (1u + P.move_chunks), *flag = ticket + 1;
+  if (tid == 0)
+    s_chunk = atomicAdd(ticket, 1u);
+  __syncthreads();
+  const uint32_t rows = kMove / units, chunk = s_chunk, j0 = chunk * rows * kFewUnits;
+  if (j0 >= q.m)
+    return;
+  uint8_t *pool = vals ? P.v + (int64_t)h * P.vhs * eb : P.k + (int64_t)h * P.khs * eb;
+  const int64_t ps_b = (vals ? P.vps : P.kps) * eb, ts_b = (vals ? P.vts : P.kts) * eb;
+  const float *scale = vals ? P.vs : P.ks;
+  const float *ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
+  const uint32_t cnt = min(rows * kFewUnits, q.m - j0);
+  for (uint32_t i = tid; i < cnt; i += kMove) {
+    const uint32_t j = j0 + i, src = (uint32_t)kept[j];
+    const uint32_t sb = div_ps(P, src), db = div_ps(P, j);
+    const int64_t sp = P.bt[q.row + sb], dp = P.bt[q.row + db];
+    bool moves = src != j;
+    if constexpr (FP8) {
+      const float was = scale[(sp * P.Hkv + h) * P.scale_stride], now = ns[db];
+      s_ratio[i] = was != now ? was / now : -1.f; // below 0: the codes stay
+      moves = moves || was != now;
+    }
+    s_from[i] = moves ? sp * ps_b + (int64_t)(src - sb * P.ps) * ts_b : -1;
+    s_to[i] = dp * ps_b + (int64_t)(j - db * P.ps) * ts_b;
+  }
+  __syncthreads();
+  const uint32_t rr = tid / units, off = tid % units * 16u;
+  uint4 x[kFewUnits];
+#pragma unroll
+  for (int i = 0; i < kFewUnits; ++i) {
+    const uint32_t k = (uint32_t)i * rows + rr;
+    x[i] = uint4{};
+    if (rr < rows && k < cnt && s_from[k] >= 0)
+      x[i] = *reinterpret_cast<const uint4 *>(pool + s_from[k] + off);
+  }
+#pragma unroll
+  for (int i = 0; i < kFewUnits; ++i)
+    hold(x[i]);
+  __builtin_amdgcn_s_waitcnt(kVmcnt0);
+  __syncthreads(); // the chunk is in registers: nothing to publish but that
+  if (tid == 0)
+    __hip_atomic_store(flag + chunk, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (tid < 64u)
+    for (uint32_t k = tid; k < chunk; k += 64u)
+      while (__hip_atomic_load(flag + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == 0u)
+        __builtin_amdgcn_s_sleep(1);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kFewUnits; ++i) {
+    const uint32_t k = (uint32_t)i * rows + rr;
+    if (rr < rows && k < cnt && s_from[k] >= 0) {
+      if constexpr (FP8) {
+        const float f = s_ratio[k];
+        if (f >= 0.f)
+          recode(x[i], f);
+      }
+      *reinterpret_cast<uint4 *>(pool + s_to[k] + off) = x[i];
     }
   }
 }
@@ -516,11 +894,61 @@ int check_shape(const SchedEvictArgs *a) {
   return 0;
 }
 
-// Workgroups of the move that fill the card.
-constexpr uint32_t kMoveFill = 512;
-
 uint32_t new_pages_of(const SchedEvictArgs *a) {
   return (uint32_t)(((uint64_t)a->max_keep + a->page_size - 1u) / a->page_size);
+}
+
+// Tables that reach past one workgroup's registers (evict_select<512, 24>'s 12288 tokens),
+// of fewer tasks than half the compute units, take the wide selection: 8 tasks of 65537
+// tokens 198 -> 93 us with the moves, 4 of 25820 119 -> 98; 8 of 16310, which fit, 47 -> 67.
+constexpr uint32_t kMoveFill = 512; // workgroups of the move that fill the card
+constexpr uint32_t kWideTasks = 128, kShort = 256u * 16u, kOneRead = 512u * 24u;
+
+bool wide_applies(const SchedEvictArgs *a) {
+  return (uint64_t)a->max_pages * a->page_size > kOneRead &&
+         (uint64_t)a->num_requests * a->num_kv_heads < kWideTasks;
+}
+uint32_t wide_chunks(const SchedEvictArgs *a) {
+  return (uint32_t)(((uint64_t)a->max_pages * a->page_size + kWideSpan - 1u) / kWideSpan);
+}
+uint64_t scale_bytes(const SchedEvictArgs *a) {
+  if (a->kv_dtype != SCHED_PD_FP8_E4M3)
+    return 0;
+  return ((uint64_t)a->num_requests * a->num_kv_heads * 2u * new_pages_of(a) * 4u + 255u) / 256u * 256u;
+}
+uint64_t wide_bytes(const SchedEvictArgs *a) {
+  if (!wide_applies(a))
+    return 0;
+  return (uint64_t)a->num_requests * a->num_kv_heads * (3u * kWideBins + 1u + 2u * wide_chunks(a)) * 4u;
+}
+// Rows that evict_move_few moves: in 16-byte units, 4 to kMove of them.
+bool wide_rows(const SchedEvictArgs *a) {
+  const int64_t eb = elem_bytes(a->kv_dtype);
+  auto rows16 = [&](int64_t x) { return (x * eb) % 16 == 0; };
+  return a->v_dim_stride == 1 && (a->head_dim * eb) % 16 == 0 && (uintptr_t)a->k_pool % 16 == 0 &&
+         (uintptr_t)a->v_pool % 16 == 0 && rows16(a->k_page_stride) && rows16(a->k_head_stride) &&
+         rows16(a->k_tok_stride) && rows16(a->v_page_stride) && rows16(a->v_head_stride) &&
+         rows16(a->v_tok_stride);
+}
+#ifndef MFILL
+#define MFILL 512
+#endif
+#ifndef FEWM
+#define FEWM 512
+#endif
+bool few_applies(const SchedEvictArgs *a) {
+  return 2ull * a->num_requests * a->num_kv_heads < MFILL &&
+         a->head_dim * elem_bytes(a->kv_dtype) >= 64u && a->max_keep > FEWM;
+}
+uint32_t few_chunks(const SchedEvictArgs *a) {
+  const uint32_t units = a->head_dim * elem_bytes(a->kv_dtype) / 16u;
+  const uint32_t rows = kMove / units * kFewUnits;
+  return (a->max_keep + rows - 1u) / rows;
+}
+uint64_t move_bytes(const SchedEvictArgs *a) {
+  if (!few_applies(a))
+    return 0;
+  return 2ull * a->num_requests * a->num_kv_heads * (1u + few_chunks(a)) * 4u;
 }
 
 } // namespace
@@ -538,9 +966,7 @@ void sched_evict_default_args(SchedEvictArgs *a) {
 int64_t sched_kv_evict_workspace_bytes(const SchedEvictArgs *a) {
   if (check_shape(a))
     return -1;
-  if (a->kv_dtype != SCHED_PD_FP8_E4M3)
-    return 0;
-  return (int64_t)((uint64_t)a->num_requests * a->num_kv_heads * 2u * new_pages_of(a) * 4u);
+  return (int64_t)(scale_bytes(a) + wide_bytes(a) + move_bytes(a));
 }
 
 int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
@@ -590,35 +1016,50 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   const uint32_t tasks = P.R * P.Hkv;
   const uint64_t longest = (uint64_t)a->max_pages * a->page_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (longest <= 256u * 16u)
+  const bool many = wide_applies(a), few = few_applies(a) && wide_rows(a);
+  if (few) {
+    P.moves = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->workspace) + scale_bytes(a) +
+                                           wide_bytes(a));
+    P.move_chunks = few_chunks(a);
+  }
+  if (many) {
+    P.wide = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->workspace) + scale_bytes(a));
+    P.chunks = wide_chunks(a);
+    const dim3 grid(tasks, P.chunks);
+    hipLaunchKernelGGL(wide_start, dim3(tasks), dim3(kWide), 0, s, P);
+    for (int digit = 0; digit < 3; ++digit)
+      hipLaunchKernelGGL(wide_digit, grid, dim3(kWide), 0, s, P, digit);
+    hipLaunchKernelGGL(wide_count, grid, dim3(kWide), 0, s, P);
+    hipLaunchKernelGGL(wide_keep, grid, dim3(kWide), 0, s, P);
+    if (fp8)
+      hipLaunchKernelGGL(wide_scales, dim3(tasks, std::max(1u, (a->max_keep + 767u) / 768u)), dim3(1024), 0,
+                         s, P); // (a round has 769 tokens or more)
+  } else if (longest <= kShort) {
     hipLaunchKernelGGL((evict_select<256, 16>), dim3(tasks), dim3(256), 0, s, P);
-  else
-    hipLaunchKernelGGL((evict_select<1024, 32>), dim3(tasks), dim3(1024), 0, s, P);
+  } else {
+    hipLaunchKernelGGL((evict_select<512, 24>), dim3(tasks), dim3(512), 0, s, P);
+  }
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a->max_keep > 0) {
-    auto rows16 = [&](int64_t x) { return (x * eb) % 16 == 0; };
-    const bool wide = a->v_dim_stride == 1 && (a->head_dim * eb) % 16 == 0 &&
-                      (uintptr_t)a->k_pool % 16 == 0 && (uintptr_t)a->v_pool % 16 == 0 &&
-                      rows16(P.kps) && rows16(P.khs) && rows16(P.kts) && rows16(P.vps) &&
-                      rows16(P.vhs) && rows16(P.vts);
+    const bool wide = wide_rows(a);
     const uint32_t units = wide ? a->head_dim * eb / 16u : a->head_dim;
     const int64_t k_step = wide ? 16 : eb, v_step = wide ? 16 : a->v_dim_stride * eb;
-    // few tasks: a row in up to four parts, of 64 bytes at least, for more workgroups
-    uint32_t parts = 1;
-    while (wide && parts < 4u && 2u * tasks * parts < kMoveFill && units / (2u * parts) >= 4u)
-      parts *= 2u;
-    const uint32_t part = (units + parts - 1u) / parts;
-    const dim3 grid(2u * tasks * parts), block(kMove);
-    if (wide && fp8)
-      hipLaunchKernelGGL((evict_move<uint4, true>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
+    P.row_groups = 2u * tasks * (few ? P.move_chunks : 1u);
+    const dim3 grid(P.row_groups + (many ? tasks : 0u)), block(kMove);
+    if (few && fp8)
+      hipLaunchKernelGGL(evict_move_few<true>, grid, block, 0, s, P, units, eb);
+    else if (few)
+      hipLaunchKernelGGL(evict_move_few<false>, grid, block, 0, s, P, units, eb);
+    else if (wide && fp8)
+      hipLaunchKernelGGL((evict_move<uint4, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
     else if (wide)
-      hipLaunchKernelGGL((evict_move<uint4, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint4, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
     else if (fp8)
-      hipLaunchKernelGGL((evict_move<uint8_t, true>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint8_t, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
     else if (eb == 2)
-      hipLaunchKernelGGL((evict_move<uint16_t, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint16_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
     else
-      hipLaunchKernelGGL((evict_move<uint32_t, false>), grid, block, 0, s, P, units, part, k_step, v_step, eb);
+      hipLaunchKernelGGL((evict_move<uint32_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
     e = hipGetLastError();
     if (e == hipSuccess && fp8) {
       hipLaunchKernelGGL(evict_scales, dim3(tasks), dim3(256), 0, s, P);
