@@ -12,7 +12,8 @@ levers. Both run on the HIP library only; there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
+import functools
+import struct
 
 import torch
 
@@ -21,6 +22,7 @@ import sched_abi as abi
 import sched_pd
 
 _F32 = torch.float32
+WORKSPACE = struct.Struct("@PQ")      # workspace, workspace_bytes
 
 
 def diff_lambda(q1, k1, q2, k2, init: float) -> torch.Tensor:
@@ -33,70 +35,81 @@ def diff_lambda(q1, k1, q2, k2, init: float) -> torch.Tensor:
 
 def _build(op, q, k_pool, v_pool, block_table, ctx_lens, out, out_dtype, v_layout, page_indptr,
            sm_scale, k_scale, v_scale, flags):
-    """A SchedMapsArgs of what both operators share, and the output tensor."""
+    """The checks both operators share: (what their argument blocks begin with, up to the
+    values that differ; the rest of the shared ones; the output tensor)."""
     dt = sched_pd._DT
-    if q.dtype not in dt or q.dtype.itemsize == 1:
+    qd, kd = dt.get(q.dtype), dt.get(k_pool.dtype)
+    if qd is None or qd == abi.FP8_E4M3:
         raise TypeError(f"q must be float32, bfloat16 or float16, got {q.dtype}")
-    if k_pool.dtype not in dt or v_pool.dtype != k_pool.dtype:
+    if kd is None or v_pool.dtype != k_pool.dtype:
         raise TypeError(f"pool dtypes {k_pool.dtype}, {v_pool.dtype}")
-    if k_pool.dim() != 4 or v_pool.dim() != 4:
+    ks, vs = k_pool.stride(), v_pool.stride()
+    if len(ks) != 4 or len(vs) != 4:
         raise ValueError("pools must have four dims")
     P, hkv, ps, d = k_pool.shape
-    ks, vs = k_pool.stride(), v_pool.stride()
     if ks[3] != 1:
         raise ValueError("k_pool dims must be contiguous")
     if v_layout == "tokmajor":
-        want, inner, vt, vd = (P, hkv, ps, d), vs[3], vs[2], vs[3]
+        want, vt, vd = (P, hkv, ps, d), vs[2], vs[3]
     elif v_layout == "dmajor":
-        want, inner, vt, vd = (P, hkv, d, ps), vs[3], vs[3], vs[2]
+        want, vt, vd = (P, hkv, d, ps), vs[3], vs[2]
     else:
         raise ValueError(f"v_layout {v_layout!r}")
-    if tuple(v_pool.shape) != want:
+    if v_pool.shape != want:
         raise ValueError(f"{v_layout} v_pool must be {want}, got {tuple(v_pool.shape)}")
-    if inner != 1:
+    if vs[3] != 1:
         raise ValueError("v_pool's last dim must be contiguous")
     R = ctx_lens.numel()
-    if q.dim() != 3 or q.shape[0] != R or q.shape[2] != d or not q.is_contiguous():
-        raise ValueError(f"q must be contiguous [{R}, Hq, {d}], got {tuple(q.shape)}")
+    qs = q.shape
+    if len(qs) != 3 or qs[0] != R or qs[2] != d or not q.is_contiguous():
+        raise ValueError(f"q must be contiguous [{R}, Hq, {d}], got {tuple(qs)}")
     if out is None:
-        out = torch.empty(q.shape, dtype=out_dtype or q.dtype, device=q.device)
-    if out.shape != q.shape or not out.is_contiguous():
-        raise ValueError(f"out must be contiguous {tuple(q.shape)}, got {tuple(out.shape)}")
-    if out.dtype not in dt or out.dtype.itemsize == 1:
+        out = torch.empty(qs, dtype=out_dtype or q.dtype, device=q.device)
+    if out.shape != qs or not out.is_contiguous():
+        raise ValueError(f"out must be contiguous {tuple(qs)}, got {tuple(out.shape)}")
+    od = dt.get(out.dtype)
+    if od is None or od == abi.FP8_E4M3:
         raise TypeError(f"out must be float32, bfloat16 or float16, got {out.dtype}")
-    a = abi.SchedMapsArgs(
-        abi_version=abi.MAPS_ABI_VERSION, op=op, kv_dtype=dt[k_pool.dtype], q_dtype=dt[q.dtype],
-        o_dtype=dt[out.dtype], num_requests=R, num_q_heads=q.shape[1], num_kv_heads=hkv,
-        head_dim=d, page_size=ps, flags=flags, sm_scale=0.0 if sm_scale is None else sm_scale,
-        num_pages=P, q=q.data_ptr(), out=out.data_ptr(), k_pool=k_pool.data_ptr(),
-        v_pool=v_pool.data_ptr(), k_page_stride=ks[0], k_head_stride=ks[1], k_tok_stride=ks[2],
-        v_page_stride=vs[0], v_head_stride=vs[1], v_tok_stride=vt, v_dim_stride=vd,
-        block_table=block_table.data_ptr(), ctx_lens=ctx_lens.data_ptr())
-    check_table(a, R, block_table, page_indptr, ctx_lens)
-    if a.kv_dtype == abi.FP8_E4M3:
+    stride, pages, indptr = table_of(R, block_table, page_indptr, ctx_lens)
+    ksp = vsp = 0
+    if kd == abi.FP8_E4M3:
         kv_cache.check_scales(k_scale, v_scale, P * hkv)
-        a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
         check_device(k_pool, k_scale=k_scale, v_scale=v_scale)
-    check_device(k_pool, q=q, out=out, k_pool=k_pool, v_pool=v_pool, block_table=block_table,
-                 ctx_lens=ctx_lens, page_indptr=page_indptr)
-    return a, out
+    dev = k_pool.get_device()
+    if dev < 0 or q.get_device() != dev or v_pool.get_device() != dev \
+            or block_table.get_device() != dev or ctx_lens.get_device() != dev \
+            or out.get_device() != dev or page_indptr is not None:
+        check_device(k_pool, q=q, out=out, k_pool=k_pool, v_pool=v_pool, block_table=block_table,
+                     ctx_lens=ctx_lens, page_indptr=page_indptr)
+    head = (abi.MAPS_ABI_VERSION, op, kd, qd, od, R, qs[1], hkv, d, ps, stride, pages, flags,
+            0.0 if sm_scale is None else sm_scale)
+    tail = (P, q.data_ptr(), out.data_ptr(), k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1],
+            ks[2], vs[0], vs[1], vt, vd, ksp, vsp, block_table.data_ptr(), indptr,
+            ctx_lens.data_ptr())
+    return head, tail, out
 
 
-def check_table(a, R, block_table, page_indptr, ctx_lens) -> None:
-    """Check a page table and lengths and fill in a's width and stride."""
-    for t, what in ((block_table, "block_table"), (ctx_lens, "ctx_lens"),
-                    (page_indptr, "page_indptr")):
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous int32")
+_I32 = torch.int32
+
+
+def table_of(R, block_table, page_indptr, ctx_lens) -> tuple:
+    """Check a page table and lengths; (row stride, pages it reaches, page_indptr's
+    address or 0)."""
+    if block_table.dtype != _I32 or not block_table.is_contiguous():
+        raise ValueError("block_table must be contiguous int32")
+    if ctx_lens.dtype != _I32 or not ctx_lens.is_contiguous():
+        raise ValueError("ctx_lens must be contiguous int32")
     if page_indptr is None:
-        if block_table.dim() != 2 or block_table.shape[0] != R:
+        shape = block_table.shape
+        if len(shape) != 2 or shape[0] != R:
             raise ValueError(f"block_table must be [{R}, max_pages] without page_indptr")
-        a.bt_stride = a.max_pages = block_table.shape[1]
-    else:
-        if page_indptr.numel() != R + 1:
-            raise ValueError("page_indptr needs num_requests + 1 entries")
-        a.max_pages = block_table.numel()
-        a.page_indptr = page_indptr.data_ptr()
+        return shape[1], shape[1], 0
+    if page_indptr.dtype != _I32 or not page_indptr.is_contiguous():
+        raise ValueError("page_indptr must be contiguous int32")
+    if page_indptr.numel() != R + 1:
+        raise ValueError("page_indptr needs num_requests + 1 entries")
+    return 0, block_table.numel(), page_indptr.data_ptr()
 
 
 def check_device(like, **tensors) -> None:
@@ -111,7 +124,7 @@ def check_device(like, **tensors) -> None:
 
 def check_weights(weights, P, hkv, ps, what="weights") -> None:
     """Raise unless `weights` holds one fp32 per (page, kv-head, slot)."""
-    if weights.dtype != _F32 or tuple(weights.shape) != (P, hkv, ps) or weights.stride(2) != 1:
+    if weights.dtype != _F32 or weights.shape != (P, hkv, ps) or weights.stride(2) != 1:
         raise ValueError(f"{what} must be float32 [{P}, {hkv}, {ps}] with contiguous slots, got "
                          f"{weights.dtype} {tuple(weights.shape)}")
 
@@ -133,18 +146,15 @@ def scratch(need: int, workspace, device):
 
 
 def on_device(fn):
-    """Run fn(pool-like third tensor ...) with that tensor's GPU current and, if given,
-    `stream` current there, so that allocations and the launch are ordered on it."""
-    import functools
-
+    """Run fn with its first tensor's GPU current and, if given, `stream` current there, so
+    that allocations and the launch are ordered on it."""
     @functools.wraps(fn)
     def run(*args, stream=None, **kw):
-        t = args[1] if len(args) > 1 else None
-        other = isinstance(t, torch.Tensor) and t.is_cuda \
-            and t.device.index != torch._C._cuda_getDevice()
-        if stream is None and not other:
+        t = args[0] if args else next((v for v in kw.values() if isinstance(v, torch.Tensor)), None)
+        dev = t.get_device() if isinstance(t, torch.Tensor) else -1
+        if stream is None and (dev < 0 or dev == torch._C._cuda_getDevice()):
             return fn(*args, **kw)
-        with torch.cuda.device(t.device if isinstance(t, torch.Tensor) and t.is_cuda else None):
+        with torch.cuda.device(dev):
             if stream is None:
                 return fn(*args, **kw)
             with torch.cuda.stream(stream):
@@ -152,14 +162,14 @@ def on_device(fn):
     return run
 
 
-def _launch(a, workspace, device) -> None:
-    lib = abi.load_library()
-    need = lib.sched_decode_maps_workspace_bytes(ctypes.byref(a))
+def _launch(block, workspace, device) -> None:
+    """Launch a SchedMapsArgs block but for its last two fields, the workspace."""
+    need = abi.entry("sched_decode_maps_workspace_bytes")(block + bytes(16))
     if need < 0:
         raise RuntimeError(f"sched_decode_maps failed: {abi.last_error()}")
     ws = scratch(need, workspace, device)
-    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    rc = lib.sched_decode_maps(ctypes.byref(a), sched_pd._raw_stream(None))
+    rc = abi.entry("sched_decode_maps")(
+        block + WORKSPACE.pack(ws.data_ptr(), ws.numel() * ws.element_size()), sched_pd._raw_stream(None))
     if rc != 0:
         raise RuntimeError(f"sched_decode_maps failed ({rc}): {abi.last_error()}")
 
@@ -183,19 +193,22 @@ def paged_decode_weighted(q, k_pool, v_pool, block_table, ctx_lens, weights, *, 
     `stream`: the stream the call's work goes to (default: the current one).
     `workspace`: scratch of sched_decode_maps_workspace_bytes (default: taken from
     torch's allocator)."""
-    a, out = _build(abi.MAPS_WEIGHTED, q, k_pool, v_pool, block_table, ctx_lens, out, out_dtype,
-                    v_layout, page_indptr, sm_scale, k_scale, v_scale, flags)
-    check_weights(weights, a.num_pages, a.num_kv_heads, a.page_size)
-    a.decay = decay
-    a.weights = weights.data_ptr()
-    a.w_page_stride, a.w_head_stride = weights.stride(0), weights.stride(1)
+    head, tail, out = _build(abi.MAPS_WEIGHTED, q, k_pool, v_pool, block_table, ctx_lens, out,
+                             out_dtype, v_layout, page_indptr, sm_scale, k_scale, v_scale, flags)
+    P, hkv, ps, _ = k_pool.shape
+    check_weights(weights, P, hkv, ps)
+    cnt = 0
     if counted is not None:
-        if counted.dtype != torch.int32 or not counted.is_contiguous() \
-                or counted.numel() != a.num_requests:
-            raise ValueError(f"counted must be contiguous int32 [{a.num_requests}]")
-        a.counted = counted.data_ptr()
-    check_device(k_pool, weights=weights, counted=counted)
-    _launch(a, workspace, k_pool.device)
+        if counted.dtype != _I32 or not counted.is_contiguous() \
+                or counted.numel() != ctx_lens.numel():
+            raise ValueError(f"counted must be contiguous int32 [{ctx_lens.numel()}]")
+        cnt = counted.data_ptr()
+    dev = k_pool.get_device()
+    if dev < 0 or weights.get_device() != dev or (cnt and counted.get_device() != dev):
+        check_device(k_pool, weights=weights, counted=counted)
+    ws = weights.stride()
+    _launch(abi.packer(abi.SchedMapsArgs, 2)(*head, decay, 0.0, 0.0, *tail, weights.data_ptr(),
+                                             ws[0], ws[1], cnt, 0, 0), workspace, k_pool.device)
     return out
 
 
@@ -214,17 +227,18 @@ def paged_decode_diff(q, k_pool, v_pool, block_table, ctx_lens, lam, *, norm_wei
     norm_weight: float32 [d], or None for out = out_scale * o. A PagedKvCache of
     head_dim d holds such a layer as it is. A request without tokens gives NaN rows.
     `stream` and `workspace` as paged_decode_weighted's."""
-    a, out = _build(abi.MAPS_DIFF, q, k_pool, v_pool, block_table, ctx_lens, out, out_dtype,
-                    v_layout, page_indptr, sm_scale, k_scale, v_scale, flags)
-    for t, n, what in ((lam, a.num_q_heads, "lam"), (norm_weight, a.head_dim, "norm_weight")):
+    head, tail, out = _build(abi.MAPS_DIFF, q, k_pool, v_pool, block_table, ctx_lens, out,
+                             out_dtype, v_layout, page_indptr, sm_scale, k_scale, v_scale, flags)
+    _, hq, d = q.shape
+    for t, n, what in ((lam, hq, "lam"), (norm_weight, d, "norm_weight")):
         if t is not None and (t.dtype != _F32 or not t.is_contiguous() or t.numel() != n):
             raise ValueError(f"{what} must be contiguous float32 [{n}]")
-    check_device(k_pool, lam=lam, norm_weight=norm_weight)
-    a.eps, a.out_scale = eps, out_scale
-    a.lam = lam.data_ptr()
-    if norm_weight is not None:
-        a.norm_weight = norm_weight.data_ptr()
-    _launch(a, workspace, k_pool.device)
+    nw = 0 if norm_weight is None else norm_weight.data_ptr()
+    dev = k_pool.get_device()
+    if dev < 0 or lam.get_device() != dev or (nw and norm_weight.get_device() != dev):
+        check_device(k_pool, lam=lam, norm_weight=norm_weight)
+    _launch(abi.packer(abi.SchedMapsArgs, 2)(*head, 0.0, eps, out_scale, *tail, 0, 0, 0, 0,
+                                             lam.data_ptr(), nw), workspace, k_pool.device)
     return out
 
 
@@ -235,9 +249,10 @@ def kernel_kind(q, k_pool, v_pool, block_table, ctx_lens, *, diff=False, v_layou
     fp8 = k_pool.dtype.itemsize == 1
     n = k_pool.shape[0] * k_pool.shape[1]
     s = torch.empty(n, device=k_pool.device) if fp8 else None
-    a, _ = _build(op, q, k_pool, v_pool, block_table, ctx_lens, None, None, v_layout, None, None,
-                  s, s, flags)
-    kind = abi.load_library().sched_decode_maps_kernel_kind(ctypes.byref(a))
+    head, tail, _ = _build(op, q, k_pool, v_pool, block_table, ctx_lens, None, None, v_layout,
+                           None, None, s, s, flags)
+    kind = abi.entry("sched_decode_maps_kernel_kind")(
+        abi.packer(abi.SchedMapsArgs)(*head, 0.0, 0.0, 0.0, *tail, 0, 0, 0, 0, 0, 0, 0, 0))
     if kind < 0:
         raise RuntimeError(abi.last_error())
     return {0: "valu", 1: "mfma"}[kind]

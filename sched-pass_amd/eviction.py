@@ -6,14 +6,13 @@ up. Runs on the HIP library only; there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 import kv_cache
 import sched_abi as abi
 import sched_pd
-from decode_maps import check_device, check_table, check_weights, on_device, scratch
+from decode_maps import (WORKSPACE, check_device, check_weights, on_device, scratch,
+                         table_of)
 
 
 @on_device
@@ -38,71 +37,70 @@ def evict(k_pool, v_pool, weights, block_table, ctx_lens, keep_lens, *, sink=0, 
     outside the pool is left alone, its kept rows -1, counted once per kv-head in
     `errors` (int32 [1], optional). Pages of one call belong to one request each.
     `stream`: where the work goes (default: the current stream)."""
-    dt = sched_pd._DT
-    if k_pool.dtype not in dt or v_pool.dtype != k_pool.dtype:
+    kd = sched_pd._DT.get(k_pool.dtype)
+    if kd is None or v_pool.dtype != k_pool.dtype:
         raise TypeError(f"pool dtypes {k_pool.dtype}, {v_pool.dtype}")
-    if k_pool.dim() != 4 or v_pool.dim() != 4:
+    ks, vs = k_pool.stride(), v_pool.stride()
+    if len(ks) != 4 or len(vs) != 4:
         raise ValueError("pools must have four dims")
     P, hkv, ps, d = k_pool.shape
-    ks, vs = k_pool.stride(), v_pool.stride()
     if v_layout not in ("tokmajor", "dmajor"):
         raise ValueError(f"v_layout {v_layout!r}")
     tok = v_layout == "tokmajor"
     want = (P, hkv, ps, d) if tok else (P, hkv, d, ps)
-    if tuple(v_pool.shape) != want:
+    if v_pool.shape != want:
         raise ValueError(f"{v_layout} v_pool must be {want}, got {tuple(v_pool.shape)}")
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("the pools' last dims must be contiguous")
     check_weights(weights, P, hkv, ps)
+    ws = weights.stride()
     if weights_out is None:
         weights_out = weights
     else:
         check_weights(weights_out, P, hkv, ps, "weights_out")
-        if weights_out.stride() != weights.stride():
+        if weights_out.stride() != ws:
             raise ValueError("weights_out must have the strides of weights")
     if sink < 0 or recent < 0:
         raise ValueError(f"sink {sink} and recent {recent} must not be negative")
     R = ctx_lens.numel()
     if keep_lens.dtype != torch.int32 or not keep_lens.is_contiguous() or keep_lens.numel() != R:
         raise ValueError(f"keep_lens must be contiguous int32 [{R}]")
-    a = abi.SchedEvictArgs(
-        abi_version=abi.EVICT_ABI_VERSION, kv_dtype=dt[k_pool.dtype], num_requests=R,
-        num_kv_heads=hkv, head_dim=d, page_size=ps, sink=sink, recent=recent, num_pages=P,
-        k_pool=k_pool.data_ptr(), v_pool=v_pool.data_ptr(), k_page_stride=ks[0],
-        k_head_stride=ks[1], k_tok_stride=ks[2], v_page_stride=vs[0], v_head_stride=vs[1],
-        v_tok_stride=vs[2] if tok else vs[3], v_dim_stride=vs[3] if tok else vs[2],
-        weights=weights.data_ptr(), weights_out=weights_out.data_ptr(),
-        w_page_stride=weights.stride(0), w_head_stride=weights.stride(1),
-        block_table=block_table.data_ptr(), ctx_lens=ctx_lens.data_ptr(),
-        keep_lens=keep_lens.data_ptr())
-    check_table(a, R, block_table, page_indptr, ctx_lens)
-    if max_keep is None:
-        max_keep = a.max_pages * ps
-    a.max_keep = max_keep = int(max_keep)
+    stride, pages, indptr = table_of(R, block_table, page_indptr, ctx_lens)
+    max_keep = pages * ps if max_keep is None else int(max_keep)
     if kept is None:
         kept = torch.empty(R, hkv, max_keep, dtype=torch.int32, device=k_pool.device)
-    elif kept.dtype != torch.int32 or tuple(kept.shape) != (R, hkv, max_keep) \
-            or not kept.is_contiguous():
+    elif kept.dtype != torch.int32 or kept.shape != (R, hkv, max_keep) or not kept.is_contiguous():
         raise ValueError(f"kept must be contiguous int32 [{R}, {hkv}, {max_keep}]")
-    a.kept = kept.data_ptr()
-    if a.kv_dtype == abi.FP8_E4M3:
+    ksp = vsp = err = 0
+    if kd == abi.FP8_E4M3:
         kv_cache.check_scales(k_scale, v_scale, P * hkv)
-        a.k_scale, a.v_scale = k_scale.data_ptr(), v_scale.data_ptr()
+        ksp, vsp = k_scale.data_ptr(), v_scale.data_ptr()
         check_device(k_pool, k_scale=k_scale, v_scale=v_scale)
     if errors is not None:
         if errors.dtype not in (torch.int32, torch.uint32) or errors.numel() < 1:
             raise ValueError("errors must be a 32-bit integer tensor")
-        a.errors = errors.data_ptr()
-    check_device(k_pool, k_pool=k_pool, v_pool=v_pool, weights=weights, weights_out=weights_out,
-                 block_table=block_table, page_indptr=page_indptr, ctx_lens=ctx_lens,
-                 keep_lens=keep_lens, kept=kept, errors=errors)
-    lib = abi.load_library()
-    need = lib.sched_kv_evict_workspace_bytes(ctypes.byref(a))
+        err = errors.data_ptr()
+    dev = k_pool.get_device()
+    if dev < 0 or v_pool.get_device() != dev or weights.get_device() != dev \
+            or weights_out.get_device() != dev or block_table.get_device() != dev \
+            or ctx_lens.get_device() != dev or keep_lens.get_device() != dev \
+            or kept.get_device() != dev or indptr or err:
+        check_device(k_pool, k_pool=k_pool, v_pool=v_pool, weights=weights,
+                     weights_out=weights_out, block_table=block_table, page_indptr=page_indptr,
+                     ctx_lens=ctx_lens, keep_lens=keep_lens, kept=kept, errors=errors)
+    block = abi.packer(abi.SchedEvictArgs, 2)(
+        abi.EVICT_ABI_VERSION, kd, R, hkv, d, ps, stride, pages, max_keep, sink, recent, 0, P,
+        k_pool.data_ptr(), v_pool.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1],
+        vs[2] if tok else vs[3], vs[3] if tok else vs[2], ksp, vsp, weights.data_ptr(),
+        weights_out.data_ptr(), ws[0], ws[1], block_table.data_ptr(), indptr, ctx_lens.data_ptr(),
+        keep_lens.data_ptr(), kept.data_ptr(), err)
+    need = abi.entry("sched_kv_evict_workspace_bytes")(block + bytes(16))
     if need < 0:
         raise RuntimeError(abi.last_error())
+    at = size = 0
     if need:
-        ws = scratch(need, workspace, k_pool.device)
-        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel() * ws.element_size()
-    if lib.sched_kv_evict(ctypes.byref(a), sched_pd._raw_stream(None)) != 0:
+        scr = scratch(need, workspace, k_pool.device)
+        at, size = scr.data_ptr(), scr.numel() * scr.element_size()
+    if abi.entry("sched_kv_evict")(block + WORKSPACE.pack(at, size), sched_pd._raw_stream(None)) != 0:
         raise RuntimeError(abi.last_error())
     return kept

@@ -14,14 +14,12 @@ rot pass through. Runs on the HIP library only; there is no CPU path.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 import kv_cache
 import sched_abi as abi
 import sched_pd
-from decode_maps import check_device, check_table, on_device
+from decode_maps import check_device, on_device, table_of
 
 _DT = {torch.float32: abi.F32, torch.bfloat16: abi.BF16, torch.float16: abi.F16}
 
@@ -36,60 +34,79 @@ def cos_sin_table(max_pos: int, rot_dim: int, base: float = 10000.0, device="cud
     return torch.cat([ang.cos(), ang.sin()], 1).float().to(device)
 
 
-def _build(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, errors):
-    """A SchedRotaryArgs of the rows and the rotation, and the query output."""
-    if q.dtype not in _DT or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
+_ROWS = (0,) * 17        # the block's cache fields without a cache
+
+
+def _call(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out, errors,
+          cache=_ROWS):
+    """Check the rows and the rotation, launch, and return q_out. `cache`: the block's
+    last fields; without one the key rows go to k_out."""
+    dt = _DT.get(q.dtype)
+    if dt is None or k.dtype != q.dtype or (v is not None and v.dtype != q.dtype):
         raise TypeError(f"rows must all be float32, bfloat16 or float16, got {q.dtype}, {k.dtype}"
                         f"{'' if v is None else f', {v.dtype}'}")
-    if q.dim() != 3 or k.dim() != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
-        raise ValueError(f"rows must be q [T, Hq, d] and k [T, Hkv, d], got {tuple(q.shape)} and "
-                         f"{tuple(k.shape)}")
-    if v is not None and v.shape != k.shape:
-        raise ValueError(f"v must be {tuple(k.shape)}, got {tuple(v.shape)}")
-    T, hq, d = q.shape
+    qsh, ksh = q.shape, k.shape
+    if len(qsh) != 3 or len(ksh) != 3 or qsh[0] != ksh[0] or qsh[2] != ksh[2]:
+        raise ValueError(f"rows must be q [T, Hq, d] and k [T, Hkv, d], got {tuple(qsh)} and "
+                         f"{tuple(ksh)}")
+    T, hq, d = qsh
+    qs, ks = q.stride(), k.stride()
+    vp, vs = 0, (0, 0, 1)
+    if v is not None:
+        if v.shape != ksh:
+            raise ValueError(f"v must be {tuple(ksh)}, got {tuple(v.shape)}")
+        vp, vs = v.data_ptr(), v.stride()
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    elif q_out.shape != q.shape or q_out.dtype != q.dtype:
-        raise ValueError(f"q_out must be {q.dtype} {tuple(q.shape)}")
-    qs, ks, qo = q.stride(), k.stride(), q_out.stride()
-    if qs[2] != 1 or ks[2] != 1 or qo[2] != 1 or (v is not None and v.stride(2) != 1):
+        q_out = torch.empty(qsh, dtype=q.dtype, device=q.device)
+    elif q_out.shape != qsh or q_out.dtype != q.dtype:
+        raise ValueError(f"q_out must be {q.dtype} {tuple(qsh)}")
+    qo = q_out.stride()
+    if qs[2] != 1 or ks[2] != 1 or qo[2] != 1 or vs[2] != 1:
         raise ValueError("row dims must be contiguous")
-    if positions.dtype not in (torch.int32, torch.int64) or positions.numel() != T \
+    i64 = positions.dtype == torch.int64
+    if not (i64 or positions.dtype == torch.int32) or positions.numel() != T \
             or not positions.is_contiguous():
         raise ValueError(f"positions must be contiguous int32 or int64 [{T}]")
-    if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or cos_sin.stride(1) != 1:
+    cs = cos_sin.stride()
+    if cos_sin.dtype != torch.float32 or len(cs) != 2 or cs[1] != 1:
         raise ValueError("cos_sin must be float32 [max_pos, rot_dim] with contiguous rows")
-    a = abi.SchedRotaryArgs(
-        abi_version=abi.ROTARY_ABI_VERSION, dtype=_DT[q.dtype], num_tokens=T, num_q_heads=hq,
-        num_kv_heads=k.shape[1], head_dim=d, rot_dim=cos_sin.shape[1],
-        interleaved=1 if interleaved else 0, pos_i64=positions.dtype == torch.int64,
-        max_pos=cos_sin.shape[0], eps=eps, q=q.data_ptr(), k=k.data_ptr(), q_tok_stride=qs[0],
-        q_head_stride=qs[1], k_tok_stride=ks[0], k_head_stride=ks[1], q_out=q_out.data_ptr(),
-        qo_tok_stride=qo[0], qo_head_stride=qo[1], positions=positions.data_ptr(),
-        cos_sin=cos_sin.data_ptr(), cs_stride=cos_sin.stride(0))
-    for w, what in ((q_weight, "q_weight"), (k_weight, "k_weight")):
-        if w is not None and (w.dtype not in _DT or w.numel() != d or not w.is_contiguous()):
-            raise ValueError(f"{what} must be contiguous [{d}]")
-    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
-        raise TypeError(f"weights of two types: {q_weight.dtype}, {k_weight.dtype}")
-    w = q_weight if q_weight is not None else k_weight
-    a.w_dtype = abi.F32 if w is None else _DT[w.dtype]
+    qw = kw = wd = 0
     if q_weight is not None:
-        a.q_weight = q_weight.data_ptr()
+        qw, wd = _weight(q_weight, d, "q_weight")
     if k_weight is not None:
-        a.k_weight = k_weight.data_ptr()
+        kw, kd = _weight(k_weight, d, "k_weight")
+        if qw and kd != wd:
+            raise TypeError(f"weights of two types: {q_weight.dtype}, {k_weight.dtype}")
+        wd = kd
+    err = 0
     if errors is not None:
         if errors.dtype not in (torch.int32, torch.uint32) or errors.numel() < 1:
             raise ValueError("errors must be a 32-bit integer tensor")
-        a.errors = errors.data_ptr()
-    check_device(k, q=q, v=v, q_out=q_out, positions=positions, cos_sin=cos_sin,
-                 q_weight=q_weight, k_weight=k_weight, errors=errors)
-    return a, q_out
-
-
-def _launch(a) -> None:
-    if abi.load_library().sched_qk_norm_rope(ctypes.byref(a), sched_pd._raw_stream(None)) != 0:
+        err = errors.data_ptr()
+    dev = k.get_device()
+    if dev < 0 or q.get_device() != dev or positions.get_device() != dev \
+            or cos_sin.get_device() != dev or q_out.get_device() != dev \
+            or (vp and v.get_device() != dev) or (qw and q_weight.get_device() != dev) \
+            or (kw and k_weight.get_device() != dev) or err:
+        check_device(k, q=q, v=v, q_out=q_out, positions=positions, cos_sin=cos_sin,
+                     q_weight=q_weight, k_weight=k_weight, errors=errors)
+    kop, ko = (0, (0, 0)) if k_out is None else (k_out.data_ptr(), k_out.stride())
+    block = abi.packer(abi.SchedRotaryArgs)(
+        abi.ROTARY_ABI_VERSION, dt, wd, T, hq, ksh[1], d, cos_sin.shape[1],
+        1 if interleaved else 0, i64, cos_sin.shape[0], eps, q.data_ptr(), k.data_ptr(), vp, qs[0],
+        qs[1], ks[0], ks[1], vs[0], vs[1], q_out.data_ptr(), kop, qo[0], qo[1], ko[0], ko[1], qw,
+        kw, positions.data_ptr(), cos_sin.data_ptr(), cs[0], err, *cache)
+    if abi.entry("sched_qk_norm_rope")(block, sched_pd._raw_stream(None)) != 0:
         raise RuntimeError(abi.last_error())
+    return q_out
+
+
+def _weight(w, d, what) -> tuple:
+    """(address, type) of a norm's weight."""
+    dt = _DT.get(w.dtype)
+    if dt is None or w.numel() != d or not w.is_contiguous():
+        raise ValueError(f"{what} must be contiguous [{d}]")
+    return w.data_ptr(), dt
 
 
 @on_device
@@ -101,17 +118,13 @@ def qk_norm_rope(q, k, positions, cos_sin, *, q_weight=None, k_weight=None, eps=
     the inputs. A token whose position lies outside cos_sin is not written and
     counted in `errors` (int32 [1], optional). `stream`: where the work goes
     (default: the current stream)."""
-    a, q_out = _build(q, k, None, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out,
-                      errors)
     if k_out is None:
         k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     elif k_out.shape != k.shape or k_out.dtype != k.dtype or k_out.stride(2) != 1 \
             or k_out.device != k.device:
         raise ValueError(f"k_out must be {k.dtype} {tuple(k.shape)} on {k.device}, dims contiguous")
-    a.k_out = k_out.data_ptr()
-    a.ko_tok_stride, a.ko_head_stride = k_out.stride(0), k_out.stride(1)
-    _launch(a)
-    return q_out, k_out
+    return _call(q, k, None, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out,
+                 k_out, errors), k_out
 
 
 @on_device
@@ -130,15 +143,8 @@ def append_rotated(q, k, v, positions, cos_sin, append_indptr, ctx_lens, k_pool,
     the rows' type in between. `errors` counts tokens with a position outside cos_sin
     and (token, kv-head) pairs that have no place in the cache."""
     if k_pool.dtype != q.dtype or v_layout != "tokmajor" or k_pool.dim() != 4:
-        if errors is not None and errors.dtype not in (torch.int32, torch.uint32):
-            raise ValueError("errors must be a 32-bit integer tensor")
-        a = kv_cache.build_append_args(
-            k, v, append_indptr, ctx_lens, k_pool, v_pool, block_table, page_indptr=page_indptr,
-            v_layout=v_layout, k_scale=k_scale, v_scale=v_scale, max_append=max_append,
-            errors=errors) if k.stride() == v.stride() else None
         q_out, k_rot = qk_norm_rope(q, k, positions, cos_sin, q_weight=q_weight, k_weight=k_weight,
                                     eps=eps, interleaved=interleaved, q_out=q_out, errors=errors)
-        del a
         kv_cache.append(k_rot, v.contiguous(), append_indptr, ctx_lens, k_pool, v_pool,
                         block_table, page_indptr=page_indptr, v_layout=v_layout, k_scale=k_scale,
                         v_scale=v_scale, max_append=max_append, errors=errors)
@@ -147,27 +153,23 @@ def append_rotated(q, k, v, positions, cos_sin, append_indptr, ctx_lens, k_pool,
     if v_pool.dtype != k_pool.dtype or v_pool.shape != k_pool.shape:
         raise ValueError(f"token-major v_pool must be {k_pool.dtype} {tuple(k_pool.shape)}, got "
                          f"{v_pool.dtype} {tuple(v_pool.shape)}")
-    if tuple(k.shape[1:]) != (hkv, d):
+    if k.shape[1:] != (hkv, d):
         raise ValueError(f"k {tuple(k.shape)} vs pool heads/dims ({hkv}, {d})")
     ks, vs = k_pool.stride(), v_pool.stride()
     if ks[3] != 1 or vs[3] != 1:
         raise ValueError("pool dims must be contiguous")
-    a, q_out = _build(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out,
-                      errors)
     R = ctx_lens.numel()
-    check_table(a, R, block_table, page_indptr, ctx_lens)
+    stride, _, indptr = table_of(R, block_table, page_indptr, ctx_lens)
     if append_indptr.dtype != torch.int32 or not append_indptr.is_contiguous() \
             or append_indptr.numel() != R + 1:
         raise ValueError("append_indptr must be contiguous int32 [num_requests + 1]")
-    check_device(k, append_indptr=append_indptr, ctx_lens=ctx_lens, k_pool=k_pool, v_pool=v_pool,
-                 block_table=block_table, page_indptr=page_indptr)
-    a.v = v.data_ptr()
-    a.v_tok_stride, a.v_head_stride = v.stride(0), v.stride(1)
-    a.num_requests, a.page_size, a.max_append, a.num_pages = R, ps, int(max_append), P
-    a.append_indptr, a.ctx_lens = append_indptr.data_ptr(), ctx_lens.data_ptr()
-    a.block_table = block_table.data_ptr()
-    a.k_pool, a.v_pool = k_pool.data_ptr(), v_pool.data_ptr()
-    a.kp_page_stride, a.kp_head_stride, a.kp_tok_stride = ks[:3]
-    a.vp_page_stride, a.vp_head_stride, a.vp_tok_stride = vs[:3]
-    _launch(a)
-    return q_out
+    dev = k.get_device()
+    if dev < 0 or k_pool.get_device() != dev or v_pool.get_device() != dev \
+            or append_indptr.get_device() != dev or ctx_lens.get_device() != dev \
+            or block_table.get_device() != dev or indptr:
+        check_device(k, append_indptr=append_indptr, ctx_lens=ctx_lens, k_pool=k_pool,
+                     v_pool=v_pool, block_table=block_table, page_indptr=page_indptr)
+    return _call(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, None,
+                 errors, (R, ps, stride, int(max_append), P, append_indptr.data_ptr(),
+                          ctx_lens.data_ptr(), block_table.data_ptr(), indptr, k_pool.data_ptr(),
+                          v_pool.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]))
