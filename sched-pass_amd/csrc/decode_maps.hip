@@ -440,15 +440,15 @@ int check_shape(const SchedMapsArgs *a) {
   return 0;
 }
 
-// The matrix cores: 16-bit caches with queries of their type, fp8 ones with bf16
+// The matrix cores: fp32 and 16-bit caches with queries of their type, fp8 ones with bf16
 // queries, rows that 16-byte loads reach, and lane offsets within 32 bits.
 bool mfma_applies(const SchedMapsArgs *a) {
-  if ((a->flags & SCHED_PD_FLAG_FORCE_VALU) || a->kv_dtype == SCHED_PD_F32 || a->head_dim == 32)
+  if ((a->flags & SCHED_PD_FLAG_FORCE_VALU) || a->head_dim == 32)
     return false;
   const bool fp8 = a->kv_dtype == SCHED_PD_FP8_E4M3;
   if (a->q_dtype != (fp8 ? SCHED_PD_BF16 : a->kv_dtype))
     return false;
-  const int64_t eb = fp8 ? 1 : 2;
+  const int64_t eb = elem_bytes(a->kv_dtype);
   const bool vt = a->v_dim_stride == 1;
   const int64_t vrow = (vt ? a->v_tok_stride : a->v_dim_stride) * eb, krow = a->k_tok_stride * eb;
   for (int64_t s : {a->k_page_stride * eb, a->k_head_stride * eb, krow, a->v_page_stride * eb,
@@ -470,7 +470,12 @@ bool mfma_applies(const SchedMapsArgs *a) {
 // 128 84.4: more than one round of workgroups) or kMostItems of the call. On the matrix
 // cores a weighted chunk's scores fit kScoreBytes of LDS (64 lognormal contexts up to 4000:
 // 32 KB 81.7, 40 77.5, 48 83.5; 64 x 2048: 32 KB cut in two, 107, 40 90.3).
+// Rows of 512 bytes and more: at least 128 tokens (two requests of 1000, 256 dims of bf16:
+// 256 tokens 14.6, 128 12.6), fp32 ones at 4 tokens a task (8, 4 and 2: 16 fp32 requests up
+// to 2000 43.1 / 29.5 / 32.9, 40 differential ones up to 1500 of 256 dims 90 / 75 / 78, 64 x
+// 1000 36.2 / 36.2 / 44.1).
 constexpr uint64_t kChunkPerTask = 8, kLeastChunk = 256, kMostChunk = 2048;
+constexpr uint64_t kWideRow = 512, kWideLeast = 128, kWidePerTask = 4;
 constexpr uint64_t kMostSplit = 64, kMostItems = 4096;
 constexpr uint32_t kScoreBytes = 40u << 10;
 
@@ -481,7 +486,10 @@ Plan plan_of(const SchedMapsArgs *a) {
   const bool weighted = a->op == SCHED_MAPS_WEIGHTED;
   p.mfma = mfma_applies(a);
   p.rows = a->num_q_heads / a->num_kv_heads * (weighted ? 1u : 2u);
-  uint64_t chunk = std::min(std::max(kChunkPerTask * tasks, kLeastChunk), kMostChunk);
+  const bool wide = (uint64_t)a->head_dim * elem_bytes(a->kv_dtype) >= kWideRow;
+  const uint64_t per = wide && a->kv_dtype == SCHED_PD_F32 ? kWidePerTask : kChunkPerTask;
+  uint64_t chunk = std::max(per * tasks, wide ? kWideLeast : kLeastChunk);
+  chunk = std::min(chunk, kMostChunk);
   chunk = std::max({chunk, longest / kMostSplit, longest * tasks / kMostItems});
   if (weighted && p.mfma) // a whole task may have 3/2 of it
     chunk = std::min<uint64_t>(chunk, kScoreBytes / (p.rows * 4u) * 2u / 3u);
@@ -517,11 +525,13 @@ template <typename T> StreamFn valu_of(uint32_t d, bool diff) {
 // bits at three waves spills 4 registers (64 lognormal contexts 87 us, at two 77.5); two
 // blocks of 256 dims spill 44 at two waves, and at one wave without spills take 52.3 us
 // where one block at two waves takes 48.4 (32771 tokens, the keys of the next block
-// under way while a block's values are multiplied).
+// under way while a block's values are multiplied). Blocks of fp32 are as many bytes as that
+// and go one by one: 64 dims at four waves 14.5 us, two blocks at three 16.7, four at two
+// 18.8 (96 x 30..300 tokens); 128 dims at two waves 36.2, two blocks at one 38.0 (64 x 1000).
 template <int KV, int D, bool VT, bool DIFF> StreamFn mfma_rows(uint32_t rows) {
-  constexpr bool FP8 = KV == kMapFp8;
-  constexpr int DEPTH = D == 256 ? (FP8 ? 2 : 1) : D == 128 ? (FP8 ? 3 : 2) : 4;
-  constexpr int WPE = D == 256 || (D == 128 && !FP8) ? 2 : 3;
+  constexpr bool FP8 = KV == kMapFp8, F32 = KV == kMapF32;
+  constexpr int DEPTH = F32 ? 1 : D == 256 ? (FP8 ? 2 : 1) : D == 128 ? (FP8 ? 3 : 2) : 4;
+  constexpr int WPE = F32 ? 256 / D : D == 256 || (D == 128 && !FP8) ? 2 : 3;
   return rows <= 4   ? maps_mfma<KV, D, VT, 4, DIFF, 4, DEPTH, WPE>
          : rows <= 8 ? maps_mfma<KV, D, VT, 8, DIFF, 4, DEPTH, WPE>
                      : maps_mfma<KV, D, VT, 16, DIFF, 4, DEPTH, WPE>;
@@ -626,7 +636,8 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
   const uint32_t tasks = P.R * P.Hkv;
   StreamFn fn;
   if (plan.mfma)
-    fn = a->kv_dtype == SCHED_PD_BF16  ? mfma_of<kMapBf16>(P.D, P.vds == 1, diff, P.rows)
+    fn = a->kv_dtype == SCHED_PD_F32   ? mfma_of<kMapF32>(P.D, P.vds == 1, diff, P.rows)
+         : a->kv_dtype == SCHED_PD_BF16 ? mfma_of<kMapBf16>(P.D, P.vds == 1, diff, P.rows)
          : a->kv_dtype == SCHED_PD_F16 ? mfma_of<kMapF16>(P.D, P.vds == 1, diff, P.rows)
                                        : mfma_of<kMapFp8>(P.D, P.vds == 1, diff, P.rows);
   else

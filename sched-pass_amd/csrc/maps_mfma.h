@@ -1,4 +1,4 @@
-// maps_mfma.h -- the stream of sched_decode_maps on the CDNA4 matrix cores: 16-bit or
+// maps_mfma.h -- the stream of sched_decode_maps on the CDNA4 matrix cores: fp32, 16-bit or
 // fp8 e4m3fn caches, head dims 64, 128 and 256, either V layout, up to 16 map rows.
 //
 // The tiles are decode_mfma.h's (S^T = K Q^T over 16 tokens, then O^T += V^T P^T with the
@@ -17,6 +17,11 @@
 // or 2^-37 at least). V of tokens past the context is selected to zero: 0 times what an
 // unwritten slot holds would not be 0 if that is a NaN.
 //
+// fp32 caches keep fp32 all the way, through the fp32 matrix instruction (4 dims, or 4
+// tokens, a step): a lane's 16 bytes of a key row are its dims of four steps, the lane's four
+// probabilities the tokens 4 (lane / 16) + t of step t. 8 flops a byte, a third of the rate
+// at which those bytes arrive.
+//
 // Bound by the cache's bytes.
 #pragma once
 
@@ -25,11 +30,11 @@
 
 namespace schedpd {
 
-enum MapKv { kMapBf16, kMapF16, kMapFp8 };
+enum MapKv { kMapBf16, kMapF16, kMapFp8, kMapF32 };
 
 // Registers of one 16-token block in flight.
 template <int KV, int D> struct BlockRegs {
-  static constexpr int EB = KV == kMapFp8 ? 1 : 2;
+  static constexpr int EB = KV == kMapFp8 ? 1 : KV == kMapF32 ? 4 : 2;
   static constexpr int NK = D * EB / 64;         // 16-byte K loads of a lane
   static constexpr int NV = D * EB / 64;         // 16-byte V registers of a lane
   u32x4_t k[NK], v[NV];
@@ -83,7 +88,11 @@ __device__ __forceinline__ void map_issue_v(const MapParams &P, const MapTask &T
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       const uint8_t *a = vp + t * T.vstep + T.vlane;
-      if constexpr (LB == 4) {
+      if constexpr (KV == kMapF32) { // 4 dims of each 64
+#pragma unroll
+        for (int g = 0; g < D / 64; ++g)
+          B.v[4 * g + t] = gload<true>(reinterpret_cast<const u32x4_t *>(a + 256 * g));
+      } else if constexpr (LB == 4) {
         B.v[0][t] = gload<true>(reinterpret_cast<const unsigned *>(a));
       } else if constexpr (LB == 8) {
         const u32x2_t x = gload<true>(reinterpret_cast<const u32x2_t *>(a));
@@ -104,16 +113,17 @@ __device__ __forceinline__ void map_issue_v(const MapParams &P, const MapTask &T
   }
 }
 
-template <int D> struct MapState {
+template <int KV, int D> struct MapState {
   float m, l;
   f32x4_t acc[D / 16];
-  bf16x8_t q[D / 32];
+  u32x4_t q[KV == kMapF32 ? D / 16 : D / 32]; // the lane's dims of each step, or of four
 };
 
 // The A operand of dim block blk: 4 tokens of one dim. fp8 blocks come as one dword of
 // four codes from `v8`.
 template <int KV, int D, bool VT>
 __device__ __forceinline__ s16x4_t map_v_operand(const u32x4_t *v, const unsigned *v8, int blk) {
+  static_assert(KV != kMapF32, "fp32 values are operands as they are");
   if constexpr (KV == kMapFp8)
     return __builtin_bit_cast(s16x4_t, fp8x4_to_bf16x4(v8[blk]));
   else if constexpr (!VT)
@@ -129,6 +139,8 @@ __device__ __forceinline__ s16x4_t map_v_operand(const u32x4_t *v, const unsigne
 template <int KV, int D, bool VT> __device__ __forceinline__ uint32_t map_dim(int blk, uint32_t rr) {
   if constexpr (!VT)
     return 16u * blk + rr;
+  else if constexpr (KV == kMapF32)
+    return 64u * (blk >> 2) + 4u * rr + (blk & 3);
   else if constexpr (KV != kMapFp8 && D == 256)
     return 128u * (blk >> 3) + 8u * rr + (blk & 7);
   else
@@ -140,7 +152,7 @@ constexpr float kF16P = 4096.f; // fp16 probabilities travel times this
 // One block: scores, then `next_k` (the block's keys are done with), then the softmax and
 // the products.
 template <int KV, int D, bool VT, bool DIFF, typename F>
-__device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T, MapState<D> &S,
+__device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T, MapState<KV, D> &S,
                                             const BlockRegs<KV, D> &B, uint32_t blk_in_chunk,
                                             float *s_sc, uint32_t c16, uint32_t g4, F next_k) {
   typedef BlockRegs<KV, D> R;
@@ -151,8 +163,20 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
   if constexpr (R::NK > 1)
     k_operands(kk);
   f32x4_t sc = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (KV == kMapF32) {
+    f32x4_t sd = {0.f, 0.f, 0.f, 0.f}; // two chains
 #pragma unroll
-  for (int kb = 0; kb < D / 32; ++kb) {
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; e += 2) {
+        const unsigned k0 = kk[i][e], k1 = kk[i][e + 1], q0 = S.q[i][e], q1 = S.q[i][e + 1];
+        sc = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k0), __uint_as_float(q0), sc, 0, 0, 0);
+        sd = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(k1), __uint_as_float(q1), sd, 0, 0, 0);
+      }
+    sc += sd;
+  }
+#pragma unroll
+  for (int kb = 0; kb < (KV == kMapF32 ? 0 : D / 32); ++kb) {
     bf16x8_t a;
     if constexpr (KV != kMapFp8) {
       a = __builtin_bit_cast(bf16x8_t, kk[kb]);
@@ -162,7 +186,7 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
       const u32x2_t hi = fp8x4_to_bf16x4((kb & 1) ? raw.w : raw.y);
       a = __builtin_bit_cast(bf16x8_t, u32x4_t{lo.x, lo.y, hi.x, hi.y});
     }
-    sc = mfma_qk<KV == kMapF16>(a, S.q[kb], sc);
+    sc = mfma_qk<KV == kMapF16>(a, __builtin_bit_cast(bf16x8_t, S.q[kb]), sc);
   }
   const float ks = KV == kMapFp8 ? P.scale_log2 * B.ks : P.scale_log2, vs = B.vs;
   next_k();
@@ -197,8 +221,10 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
   for (int v = 0; v < 4; ++v)
     p[v] = __builtin_amdgcn_exp2f(s[v] - mn);
   S.l += (p[0] + p[1]) + (p[2] + p[3]);
-  u32x2_t hi, lo;
-  if constexpr (KV == kMapF16) {
+  u32x2_t hi = {0u, 0u}, lo = {0u, 0u};
+  if constexpr (KV == kMapF32) {
+    // p stays fp32
+  } else if constexpr (KV == kMapF16) {
 #pragma unroll
     for (int v = 0; v < 4; ++v)
       p[v] *= kF16P;
@@ -235,7 +261,11 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
       constexpr int LB = D / 16 * R::EB;
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
-        if constexpr (LB == 4) {
+        if constexpr (KV == kMapF32) {
+#pragma unroll
+          for (int g = 0; g < D / 64; ++g)
+            vv[4 * g + t] &= mt[t];
+        } else if constexpr (LB == 4) {
           vv[0][t] &= mt[t];
         } else if constexpr (LB == 8) {
           vv[t >> 1][2 * (t & 1)] &= mt[t];
@@ -266,12 +296,18 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
         rows_transpose4(v8 + 4 * i);
       }
     }
-  } else if constexpr (!VT) {
+  } else if constexpr (!VT && KV != kMapF32) {
     bf16_v_operands(vv);
   }
   if constexpr (!VT) {
     if (!full) { // each operand now holds the lane's own four tokens
-      if constexpr (KV == kMapFp8) {
+      if constexpr (KV == kMapF32) {
+        const u32x4_t m = {0 < left ? ~0u : 0u, 1 < left ? ~0u : 0u, 2 < left ? ~0u : 0u,
+                           3 < left ? ~0u : 0u};
+#pragma unroll
+        for (int b = 0; b < R::NV; ++b)
+          vv[b] &= m;
+      } else if constexpr (KV == kMapFp8) {
         unsigned mk = 0u;
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -290,9 +326,17 @@ __device__ __forceinline__ void map_compute(const MapParams &P, const MapTask &T
   }
 #pragma unroll
   for (int b = 0; b < D / 16; ++b) {
-    const s16x4_t a = map_v_operand<KV, D, VT>(vv, v8, b);
-    S.acc[b] = mfma_pv<KV == kMapF16>(a, ph, S.acc[b]);
-    S.acc[b] = mfma_pv<KV == kMapF16>(a, pl, S.acc[b]);
+    if constexpr (KV == kMapF32) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const unsigned v = VT ? vv[4 * (b >> 2) + t][b & 3] : vv[b][t];
+        S.acc[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(v), p[t], S.acc[b], 0, 0, 0);
+      }
+    } else {
+      const s16x4_t a = map_v_operand<KV, D, VT>(vv, v8, b);
+      S.acc[b] = mfma_pv<KV == kMapF16>(a, ph, S.acc[b]);
+      S.acc[b] = mfma_pv<KV == kMapF16>(a, pl, S.acc[b]);
+    }
   }
 }
 
@@ -313,7 +357,7 @@ __device__ __forceinline__ MapBlock in_pool(const MapParams &P, MapBlock b) {
 // followed by one block's loads, page ids come a ring ahead, and a short wave re-reads its
 // last block into unused slots.
 template <int KV, int D, bool VT, bool DIFF, int NW, int DEPTH>
-__device__ __forceinline__ void map_stream(const MapParams &P, const MapTask &T, MapState<D> &S,
+__device__ __forceinline__ void map_stream(const MapParams &P, const MapTask &T, MapState<KV, D> &S,
                                            float *s_sc, uint32_t c16, uint32_t g4) {
   const int cnt = T.nblk > T.w ? (int)((T.nblk - T.w + NW - 1) / NW) : 0;
   if (cnt <= 0)
@@ -397,30 +441,32 @@ __global__ void __launch_bounds__(NW * 64) maps_mfma(MapParams P) {
   if constexpr (VT) {
     const uint32_t vrow = (uint32_t)(P.vts * EB);
     T.vsub = 16 * P.vts * EB, T.vstep = P.vts * EB;
-    T.vlane = 4u * g4 * vrow + (D * EB == 512 ? 16u : D / 16 * EB) * c16;
+    T.vlane = 4u * g4 * vrow + (D / 16 * EB > 16 ? 16u : D / 16 * EB) * c16;
   } else {
     const uint32_t vrow = (uint32_t)(P.vds * EB);
-    T.vsub = 16 * EB, T.vstep = (KV == kMapFp8 ? 64 : 32) * P.vds * EB;
-    T.vlane = KV == kMapFp8 ? (c16 + 16u * g4) * vrow
-                            : (c16 + 16u * (g4 & 1u)) * vrow + 16u * (g4 >> 1);
+    T.vsub = 16 * EB, T.vstep = (KV == kMapFp8 ? 64 : KV == kMapF32 ? 16 : 32) * P.vds * EB;
+    T.vlane = KV == kMapFp8   ? (c16 + 16u * g4) * vrow
+              : KV == kMapF32 ? c16 * vrow + 16u * g4
+                              : (c16 + 16u * (g4 & 1u)) * vrow + 16u * (g4 >> 1);
   }
   T.per = P.ps / 16u;
   T.magic = T.per == 1u ? 0u : 0xffffffffu / T.per + 1u;
 
-  MapState<D> S;
+  MapState<KV, D> S;
   S.m = kMInit, S.l = 0.f;
 #pragma unroll
   for (int b = 0; b < D / 16; ++b)
     S.acc[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
   const uint32_t hq = h * P.G + (DIFF ? c16 >> 1 : c16);
 #pragma unroll
-  for (int kb = 0; kb < D / 32; ++kb) {
-    const uint32_t d0 = qk_dim(KV == kMapFp8, kb, g4);
+  for (int i = 0; i < (KV == kMapF32 ? D / 16 : D / 32); ++i) {
+    const uint32_t d0 = KV == kMapF32 ? 16u * i + 4u * g4 : qk_dim(KV == kMapFp8, i, g4);
     u32x4_t qv = {0u, 0u, 0u, 0u};
     if (c16 < P.rows && (!DIFF || (d0 >= D / 2) == ((c16 & 1u) != 0u)))
-      qv = *reinterpret_cast<const u32x4_t *>(static_cast<const uint16_t *>(P.q) +
-                                              ((int64_t)r * P.Hq + hq) * D + d0);
-    S.q[kb] = __builtin_bit_cast(bf16x8_t, qv);
+      qv = *reinterpret_cast<const u32x4_t *>(
+          static_cast<const uint8_t *>(P.q) +
+          (((int64_t)r * P.Hq + hq) * D + d0) * (KV == kMapF32 ? 4 : 2));
+    S.q[i] = qv;
   }
 
   map_stream<KV, D, VT, DIFF, NW, DEPTH>(P, T, S, s_sc, c16, g4);

@@ -24,9 +24,10 @@ def q_of(kv):
     return torch.bfloat16 if kv == FP8 else kv
 
 
-def p_err(kind):
-    """The matrix cores take a probability as two halves of its type: within 2^-16."""
-    return 2.0 ** -16 if kind == "mfma" else 0.0
+def p_err(kind, kv):
+    """The matrix cores take a probability as two halves of a 16-bit type: within 2^-16;
+    with fp32 values as it is."""
+    return 2.0 ** -16 if kind == "mfma" and kv != torch.float32 else 0.0
 
 
 def make_q(R, hq, d, dt, seed, scale=1.0):
@@ -62,7 +63,7 @@ def check_weighted(lens, hkv, G, d, ps, kv, layout="tokmajor", seed=1, flags=0, 
     kind = decode_maps.kernel_kind(q.cuda(), x["k"], x["v"], x["bt"] if not csr else
                                    torch.zeros(len(lens), 1, dtype=torch.int32).cuda(),
                                    x["ctx"], v_layout=x["layout"], flags=flags)
-    ro, bo, rw, bw = mr.weighted_ref(c, q, w, counted, decay, p_err=p_err(kind),
+    ro, bo, rw, bw = mr.weighted_ref(c, q, w, counted, decay, p_err=p_err(kind, kv),
                                      out_dtype=out.dtype)
     mr.close(out, ro, bo, "out")
     mr.close(wg, rw, bw, "weights")
@@ -88,6 +89,25 @@ def test_weighted_head_dim_32():
 @pytest.mark.parametrize("ps", [16, 48, 256])
 def test_weighted_layouts_and_pages(kv, layout, ps):
     check_weighted(LENS, 2, 4, 128, ps, kv, layout, seed=ps)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("layout,ps", [("dmajor", 48), ("nhd", 16), ("dmajor", 16)])
+def test_weighted_fp32_layouts(d, layout, ps):
+    assert check_weighted(LENS, 2, 3, d, ps, torch.float32, layout, seed=d + ps) == "mfma"
+
+
+@pytest.mark.parametrize("kv,d", [(torch.float32, 256), (torch.bfloat16, 256), (FP8, 256),
+                                  (torch.float16, 64), (FP8, 64)])
+def test_weighted_many_chunks(kv, d):
+    """One request of some 40 chunks beside short ones, and a chunk's last token alone."""
+    check_weighted([10241, 5, 0, 257], 1, 3, d, 16, kv, seed=d)
+
+
+def test_weighted_whole_groups_of_chunks():
+    """Chunks at the edges where a task is cut or left whole."""
+    check_weighted([255, 256, 257, 383, 384, 385, 511, 512, 513], 1, 2, 128, 16, torch.bfloat16)
+    check_weighted([127, 128, 129, 191, 192, 193, 255, 256, 257], 1, 2, 128, 16, torch.float32)
 
 
 @pytest.mark.parametrize("kv", [torch.float32, torch.bfloat16, FP8])
@@ -139,7 +159,7 @@ def check_diff(lens, hkv, G, d, ps, kv, layout="tokmajor", seed=1, flags=0, csr=
     kind = decode_maps.kernel_kind(q.cuda(), x["k"], x["v"], torch.zeros(
         len(lens), 1, dtype=torch.int32).cuda(), x["ctx"], diff=True, v_layout=x["layout"],
         flags=flags)
-    ro, bo = mr.diff_ref(c, q, lam, nw, 1e-5, 0.2, sm_scale, p_err(kind), out.dtype)
+    ro, bo = mr.diff_ref(c, q, lam, nw, 1e-5, 0.2, sm_scale, p_err(kind, kv), out.dtype)
     mr.close(out, ro, bo, "out")
 
 
@@ -155,6 +175,18 @@ def test_diff_types_and_heads(kv, d, G, flags):
 @pytest.mark.parametrize("norm", [True, False])
 def test_diff_layouts(layout, ps, csr, norm):
     check_diff(LENS, 2, 2, 128, ps, torch.bfloat16, layout, seed=ps, csr=csr, norm=norm)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("layout,ps,csr", [("dmajor", 48, False), ("nhd", 16, True)])
+def test_diff_fp32_layouts(d, layout, ps, csr):
+    check_diff(LENS, 2, 3, d, ps, torch.float32, layout, seed=d, csr=csr)
+
+
+@pytest.mark.parametrize("kv,d", [(torch.float32, 256), (torch.bfloat16, 256), (FP8, 256),
+                                  (torch.float16, 64), (FP8, 64)])
+def test_diff_many_chunks(kv, d):
+    check_diff([10241, 5, 0, 257], 1, 3, d, 16, kv, seed=d)
 
 
 @pytest.mark.parametrize("lens", [[1], [9000], [130] * 40])
