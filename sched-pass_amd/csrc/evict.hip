@@ -901,7 +901,6 @@ uint32_t new_pages_of(const SchedEvictArgs *a) {
 // Tables that reach past one workgroup's registers (evict_select<512, 24>'s 12288 tokens),
 // of fewer tasks than half the compute units, take the wide selection: 8 tasks of 65537
 // tokens 198 -> 93 us with the moves, 4 of 25820 119 -> 98; 8 of 16310, which fit, 47 -> 67.
-constexpr uint32_t kMoveFill = 512; // workgroups of the move that fill the card
 constexpr uint32_t kWideTasks = 128, kShort = 256u * 16u, kOneRead = 512u * 24u;
 
 bool wide_applies(const SchedEvictArgs *a) {
@@ -930,15 +929,15 @@ bool wide_rows(const SchedEvictArgs *a) {
          rows16(a->k_tok_stride) && rows16(a->v_page_stride) && rows16(a->v_head_stride) &&
          rows16(a->v_tok_stride);
 }
-#ifndef MFILL
-#define MFILL 512
-#endif
-#ifndef FEWM
-#define FEWM 512
-#endif
+// Whether the rows are cut over workgroups. In us, with one workgroup per task and tensor
+// against chunks (head dim 128, bf16): 8 tasks of 1000 tokens 23.0 / 19.2, 192 of 1200 51.4 /
+// 48.8, 192 of 2048 fp8 47.7 / 44.9; at 256 tasks even (1200 tokens 62.1 / 62.8) or worse (2048
+// 77.7 / 81.9), and at 360 kept tokens and fewer too (8 of 300 12.9 / 13.2, 32 of 400 17.3 / 17.7).
+constexpr uint32_t kMoveFill = 512; // workgroups of evict_move that fill the card
+constexpr uint32_t kFewKeep = 512;
 bool few_applies(const SchedEvictArgs *a) {
-  return 2ull * a->num_requests * a->num_kv_heads < MFILL &&
-         a->head_dim * elem_bytes(a->kv_dtype) >= 64u && a->max_keep > FEWM;
+  return 2ull * a->num_requests * a->num_kv_heads < kMoveFill &&
+         a->head_dim * elem_bytes(a->kv_dtype) >= 64u && a->max_keep > kFewKeep;
 }
 uint32_t few_chunks(const SchedEvictArgs *a) {
   const uint32_t units = a->head_dim * elem_bytes(a->kv_dtype) / 16u;

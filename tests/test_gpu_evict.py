@@ -163,6 +163,73 @@ def test_one_long_request():
     check([20011], [20010], hkv=1, d=32, kind="ties")
 
 
+@pytest.mark.parametrize("kind", ["long", "ties", "equal", "odd", "close"])
+def test_one_read_of_a_table_of_12288_tokens(kind):
+    check([12256, 4097, 12000, 5], [6000, 4096, 11999, 3], hkv=1, d=8, sink=4, recent=64, kind=kind)
+
+
+@pytest.mark.parametrize("kind", ["long", "ties", "odd"])
+def test_stretches(kind):
+    """Tables longer than one workgroup's registers, of many tasks."""
+    lens = [30000, 12289, 24577, 13] + [50] * 124
+    check(lens, [5000, 12288, 100, 7] + [20] * 124, hkv=1, d=4, sink=2, recent=100, kind=kind)
+
+
+@pytest.mark.parametrize("kind", ["ties", "equal", "odd", "close"])
+def test_wide_orders(kind):
+    check([13000, 70, 12300, 4096, 8193], [800, 69, 12299, 4095, 4097], hkv=2, d=8, sink=3,
+          recent=33, kind=kind)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.bfloat16, FP8])
+@pytest.mark.parametrize("csr,inplace", [(False, True), (True, False)])
+def test_wide_types(kv, csr, inplace):
+    """Few long requests: the wide selection and the rows in chunks."""
+    check([12500, 90, 700], [2500, 80, 650], hkv=2, d=64, kv=kv, csr=csr, inplace=inplace, sink=1,
+          recent=50, pairs=False)
+
+
+def test_wide_without_what_is_not_cut():
+    check([12500, 90], [12500, 200], hkv=1, d=8, max_keep=13000)
+    check([12500, 90], [12500, 0], hkv=1, d=8, max_keep=13000, inplace=False)
+    check([12500, 90], [100, 90], hkv=1, d=8, sink=100, recent=100)
+
+
+@pytest.mark.parametrize("kv,d", [(torch.float32, 16), (torch.bfloat16, 32), (FP8, 64),
+                                  (FP8, 256), (torch.float32, 256), (torch.float16, 96)])
+def test_rows_in_chunks(kv, d):
+    check([2000, 700, 3], [1900, 513, 2], kv=kv, d=d, hkv=2, recent=7)
+
+
+def test_another_stream_and_few_rows_in_a_graph():
+    """Long and few: tickets and flags are cleared by every run and replay."""
+    lens, keep = [14000, 2500], [2000, 1200]
+    c = mr.paged(lens, 2, 64, 16, torch.bfloat16, seed=8)
+    w = weights_of(c, 2, 16, 8, "long")
+    kt = torch.tensor(keep, dtype=torch.int32).cuda()
+    a, b = mr.to_gpu(c), mr.to_gpu(c)
+    wa, wb = w.cuda(), w.cuda()
+
+    def cut(x, wt, **kw):
+        return eviction.evict(x["k"], x["v"], wt, x["bt"], x["ctx"], kt, recent=8, max_keep=2000,
+                              v_layout="tokmajor", **kw)
+
+    s = torch.cuda.Stream()
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            graphs.append((g, cut(a, wa)))
+    torch.cuda.synchronize()
+    for k in range(6):
+        g, kept = graphs[k % 2]
+        g.replay()
+        ref = cut(b, wb, stream=s)
+        torch.cuda.synchronize()
+        assert torch.equal(kept, ref) and torch.equal(wa, wb), k
+        assert torch.equal(bits(a["k"]), bits(b["k"])) and torch.equal(bits(a["v"]), bits(b["v"]))
+
+
 def test_a_request_with_a_bad_table_is_left_alone():
     c = mr.paged([200, 100, 90], 2, 64, 16, torch.bfloat16, seed=4)
     w = weights_of(c, 2, 16, 4, "long")

@@ -87,6 +87,36 @@ def test_counts_of_tokens(T, norm):
     mr.close(k, *ref_rows(qkv[:, 32:40], kw, pos.long(), table.cpu(), 1e-6, False))
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("d,rot", [(128, 128), (64, 32), (256, 64), (96, 96), (80, 20)])
+def test_many_tokens(dt, inter, d, rot):
+    """Enough rows that a lane has several."""
+    T, hq, hkv = 3001, 6, 2
+    qkv, qw, kw = case(T, hq, hkv, d, dt, d + rot)
+    table = rotary.cos_sin_table(4096, rot)
+    pos = torch.randint(0, 4096, (T,))
+    x = qkv.cuda()
+    q, k = rotary.qk_norm_rope(x[:, :hq], x[:, hq:hq + hkv], pos.cuda(), table, q_weight=cu(qw),
+                               k_weight=cu(kw), eps=1e-6, interleaved=inter)
+    mr.close(q, *ref_rows(qkv[:, :hq], qw, pos, table.cpu(), 1e-6, inter))
+    mr.close(k, *ref_rows(qkv[:, hq:hq + hkv], kw, pos, table.cpu(), 1e-6, inter))
+
+
+def test_on_another_stream():
+    qkv, qw, kw = case(50, 8, 2, 128, torch.bfloat16, 12)
+    table = rotary.cos_sin_table(64, 128)
+    x, pos = qkv.cuda(), torch.arange(50).cuda()
+    args = (x[:, :8], x[:, 8:10], pos, table)
+    want = rotary.qk_norm_rope(*args, q_weight=cu(qw), k_weight=cu(kw))
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        got = rotary.qk_norm_rope(*args, q_weight=cu(qw), k_weight=cu(kw))
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 @pytest.mark.parametrize("w_dtype", [torch.bfloat16, torch.float16])
 def test_weight_types_and_one_sided_norm(w_dtype):
     qkv, qw, _ = case(9, 4, 4, 128, torch.bfloat16, 3, w_dtype=w_dtype)
