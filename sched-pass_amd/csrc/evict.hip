@@ -327,7 +327,7 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
         x[i] = w0[(int64_t)P.bt[q.row + b] * P.w_ps + (t - b * P.ps)];
       }
       if (i % 8 == 7) // eight tokens' addresses at a time
-        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
     }
   };
   load(0);
@@ -621,19 +621,24 @@ __device__ __forceinline__ void hold(uint8_t &x) {
   x = (uint8_t)y;
 }
 
-// Four e4m3 codes times f, encoded anew; NaN codes as they are.
-__device__ __forceinline__ uint32_t recode4(uint32_t c, float f) {
+// Four e4m3 codes, each times its f and encoded anew; where f is below 0, and NaN codes, as
+// they are.
+__device__ __forceinline__ uint32_t recode4(uint32_t c, const float (&f)[4]) {
   typedef __attribute__((ext_vector_type(2))) float f32x2_t;
   const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
   const f32x2_t b = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-  const float q[4] = {a.x * f, a.y * f, b.x * f, b.y * f};
+  const float q[4] = {a.x * f[0], a.y * f[1], b.x * f[2], b.y * f[3]};
   uint32_t y = encode4_fp8(q);
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const uint32_t m = 0x7fu << (8 * k), all = 0xffu << (8 * k);
-    y = (c & m) == m ? (y & ~all) | (c & all) : y;
+    y = (c & m) == m || !(f[k] >= 0.f) ? (y & ~all) | (c & all) : y;
   }
   return y;
+}
+__device__ __forceinline__ uint32_t recode4(uint32_t c, float f) {
+  const float g[4] = {f, f, f, f};
+  return recode4(c, g);
 }
 __device__ __forceinline__ void recode(uint4 &x, float f) {
   x.x = recode4(x.x, f), x.y = recode4(x.y, f), x.z = recode4(x.z, f), x.w = recode4(x.w, f);
@@ -676,106 +681,250 @@ __device__ __forceinline__ void move_weights(const EParams &P, uint32_t task) {
   }
 }
 
-// U: the unit a row is moved in (16 bytes where rows are contiguous and aligned, else
-// one element); a row is `units` of them, k_step / v_step bytes apart.
-template <typename U, bool FP8>
-__global__ void __launch_bounds__(kMove) evict_move(EParams P, uint32_t units,
-                                                    int64_t k_step, int64_t v_step, uint32_t eb) {
-  constexpr int N = 4; // units of a lane and round
-  // where a row comes from (-1: it stays) and goes to; fp8: its old scale over the new one
-  __shared__ int64_t s_from[kStage], s_to[kStage];
-  __shared__ float s_ratio[FP8 ? kStage : 1];
-  const uint32_t tid = threadIdx.x;
-  if (blockIdx.x >= P.row_groups) { // the wide selection's weights
-    move_weights(P, blockIdx.x - P.row_groups);
-    return;
-  }
-  const uint32_t which = blockIdx.x;
-  const uint32_t task = which >> 1;
-  const bool vals = (which & 1u) != 0u;
-  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
-  const Req q = req_of(P, r);
-  const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
-  if (q.m == q.n || q.m == 0u || kept[0] < 0)
-    return;
-  uint8_t *pool = vals ? P.v + (int64_t)h * P.vhs * eb : P.k + (int64_t)h * P.khs * eb;
-  const int64_t ps_b = (vals ? P.vps : P.kps) * eb, ts_b = (vals ? P.vts : P.kts) * eb;
-  const float *scale = vals ? P.vs : P.ks;
-  const float *ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
-  const uint32_t e = tid % units, rr = tid / units, rows = kMove / units;
-  const bool active = rr < rows;
-  const int64_t off = (int64_t)e * (vals ? v_step : k_step);
-  const uint32_t round = rows * N;
+// How a tensor's tokens are moved: element by element, in 16-byte units of their rows, or
+// (d-major values) in 16 bytes of tokens of one dim.
+enum Mode : uint32_t { kElems, kRows, kTurned };
 
-  for (uint32_t j0 = 0; j0 < q.m; j0 += kStage) {
-    const uint32_t cnt = min(kStage, q.m - j0);
-    __syncthreads(); // the previous stage's places have been used
-    for (uint32_t i = tid; i < cnt; i += kMove) {
-      const uint32_t j = j0 + i, src = (uint32_t)kept[j];
-      const uint32_t sb = div_ps(P, src), db = div_ps(P, j);
-      const int64_t sp = P.bt[q.row + sb], dp = P.bt[q.row + db];
-      bool moves = src != j;
-      if constexpr (FP8) {
-        const float was = scale[(sp * P.Hkv + h) * P.scale_stride], now = ns[db];
-        s_ratio[i] = was != now ? was / now : -1.f; // below 0: the codes stay
-        moves = moves || was != now;
-      }
-      s_from[i] = moves ? sp * ps_b + (int64_t)(src - sb * P.ps) * ts_b : -1;
-      s_to[i] = dp * ps_b + (int64_t)(j - db * P.ps) * ts_b;
+template <int EB> struct Elem;
+template <> struct Elem<1> { typedef uint8_t type; };
+template <> struct Elem<2> { typedef uint16_t type; };
+template <> struct Elem<4> { typedef uint32_t type; };
+
+// One of a task's two tensors: where its tokens are, in bytes.
+struct Side {
+  uint8_t *pool; // the kv-head's
+  int64_t page, tok, dim;
+  const float *scale, *ns; // fp8: the pages' scales and the new ones
+};
+
+template <int EB>
+__device__ __forceinline__ Side side_of(const EParams &P, uint32_t task, uint32_t h, bool vals) {
+  Side S;
+  S.pool = (vals ? P.v + (int64_t)h * P.vhs * EB : P.k + (int64_t)h * P.khs * EB);
+  S.page = (vals ? P.vps : P.kps) * EB, S.tok = (vals ? P.vts : P.kts) * EB;
+  S.dim = (vals ? P.vds : 1) * EB;
+  S.scale = vals ? P.vs : P.ks;
+  S.ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
+  return S;
+}
+
+// The places of kept tokens j0 .. j0 + cnt - 1: from (with kStays: the token is there already,
+// as it will be), to, and for fp8 the old scale over the new one (below 0: the codes stay).
+constexpr int64_t kStays = INT64_MIN;
+template <bool FP8>
+__device__ __forceinline__ void places(const EParams &P, const Req &q, uint32_t h, const Side &S,
+                                       const int32_t *kept, uint32_t j0, uint32_t cnt,
+                                       int64_t *s_from, int64_t *s_to, float *s_ratio) {
+  for (uint32_t i = threadIdx.x; i < cnt; i += kMove) {
+    const uint32_t j = j0 + i, src = (uint32_t)kept[j];
+    const uint32_t sb = div_ps(P, src), db = div_ps(P, j);
+    const int64_t sp = P.bt[q.row + sb], dp = P.bt[q.row + db];
+    bool moves = src != j;
+    if constexpr (FP8) {
+      const float was = S.scale[(sp * P.Hkv + h) * P.scale_stride], now = S.ns[db];
+      s_ratio[i] = was != now ? was / now : -1.f;
+      moves = moves || was != now;
     }
-    __syncthreads();
-    U x[N], nx[N];
-    auto fetch = [&](uint32_t k0) __attribute__((always_inline)) {
+    s_from[i] = (sp * S.page + (int64_t)(src - sb * P.ps) * S.tok) | (moves ? 0 : kStays);
+    s_to[i] = dp * S.page + (int64_t)(j - db * P.ps) * S.tok;
+  }
+}
+
+// kTurned: 16 bytes of one dim, the values of 16 / EB tokens from k0 on (`pool` at the dim).
+// False: none of them moves. (Loads under no condition, in flight together: a token from
+// cnt on reads as the last.)
+template <int EB>
+__device__ __forceinline__ bool gather16(const uint8_t *pool, const int64_t *s_from, uint32_t k0,
+                                         uint32_t cnt, uint4 &x) {
+  typedef typename Elem<EB>::type E;
+  constexpr int TOK = 16 / EB, PER = 4 / EB; // tokens of it, and of a word
+  uint32_t w[4] = {0u, 0u, 0u, 0u};
+  bool any = false;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t k = k0 + (uint32_t)i * rows + rr;
-        nx[i] = U{};
-        if (active && k < cnt) {
-          const int64_t from = s_from[k];
-          if (from >= 0)
-            nx[i] = *reinterpret_cast<const U *>(pool + from + off);
-        }
+  for (int t = 0; t < TOK; ++t) {
+    const int64_t from = s_from[min(k0 + t, cnt - 1u)];
+    any = any || from >= 0;
+    const uint32_t e = *reinterpret_cast<const E *>(pool + (from & ~kStays));
+    w[t / PER] |= e << (8 * EB * (t % PER));
+  }
+  x = uint4{w[0], w[1], w[2], w[3]};
+  return any;
+}
+
+// Behind piece i of N: 32 of gather16's loads in flight at most (a piece's come apart in
+// registers until it is whole).
+template <int EB, int N> __device__ __forceinline__ void gather_step(int i, uint4 (&x)[N]) {
+  if (i % EB == EB - 1) {
+#pragma unroll
+    for (int j = 0; j < N; ++j)
+      if (j > i - 2 * EB && j <= i - EB)
+        hold(x[j]);
+    asm volatile("" ::: "memory");
+  }
+}
+
+template <int EB>
+__device__ __forceinline__ void scatter16(uint8_t *pool, const int64_t *s_to, const float *s_ratio,
+                                          uint32_t k0, uint32_t cnt, uint4 x) {
+  typedef typename Elem<EB>::type E;
+  constexpr int TOK = 16 / EB, PER = 4 / EB;
+  uint32_t w[4] = {x.x, x.y, x.z, x.w};
+  if constexpr (EB == 1) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float f[4];
+      bool any = false;
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        f[t] = k0 + 4 * i + t < cnt ? s_ratio[k0 + 4 * i + t] : -1.f;
+        any = any || f[t] >= 0.f;
       }
-    };
-    fetch(0);
-    for (uint32_t k0 = 0; k0 < cnt; k0 += round) {
+      if (any)
+        w[i] = recode4(w[i], f);
+    }
+  }
+  if (k0 + TOK <= cnt) {
+    *reinterpret_cast<uint4 *>(pool + s_to[k0]) = uint4{w[0], w[1], w[2], w[3]};
+  } else {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        x[i] = nx[i];
-      if (k0 + round < cnt)
-        fetch(k0 + round);
-      // this round's rows are in registers on every lane before any of them is written: each
-      // lane waits for its own here (the next round's stay under way), then the barrier
+    for (int t = 0; t < TOK; ++t)
+      if (k0 + t < cnt)
+        *reinterpret_cast<E *>(pool + s_to[k0 + t]) = (E)(w[t / PER] >> (8 * EB * (t % PER)));
+  }
+}
+
+// A stage's tokens in units U, `units` of them a token and `step` bytes apart.
+template <typename U, int N, bool FP8>
+__device__ __forceinline__ void move_units(uint8_t *pool, uint32_t units, int64_t step,
+                                           uint32_t cnt, const int64_t *s_from,
+                                           const int64_t *s_to, const float *s_ratio) {
+  const uint32_t tid = threadIdx.x, e = tid % units, rr = tid / units, rows = kMove / units;
+  const bool active = rr < rows;
+  const uint32_t round = rows * N;
+  pool += (int64_t)e * step;
+  U x[N], nx[N];
+  auto fetch = [&](uint32_t k0) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        hold(x[i]);
-      asm volatile("s_barrier" ::: "memory");
+    for (int i = 0; i < N; ++i) {
+      const uint32_t k = k0 + (uint32_t)i * rows + rr;
+      nx[i] = U{};
+      if (active && k < cnt) {
+        const int64_t from = s_from[k];
+        if (from >= 0)
+          nx[i] = *reinterpret_cast<const U *>(pool + from);
+      }
+    }
+  };
+  fetch(0);
+  for (uint32_t k0 = 0; k0 < cnt; k0 += round) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const uint32_t k = k0 + (uint32_t)i * rows + rr;
-        if (active && k < cnt && s_from[k] >= 0) {
-          if constexpr (FP8) {
-            const float f = s_ratio[k];
-            if (f >= 0.f)
-              recode(x[i], f);
-          }
-          *reinterpret_cast<U *>(pool + s_to[k] + off) = x[i];
+    for (int i = 0; i < N; ++i)
+      x[i] = nx[i];
+    if (k0 + round < cnt)
+      fetch(k0 + round);
+    // this round's rows are in registers on every lane before any of them is written: each
+    // lane waits for its own here (the next round's stay under way), then the barrier
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      hold(x[i]);
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t k = k0 + (uint32_t)i * rows + rr;
+      if (active && k < cnt && s_from[k] >= 0) {
+        if constexpr (FP8) {
+          const float f = s_ratio[k];
+          if (f >= 0.f)
+            recode(x[i], f);
         }
+        *reinterpret_cast<U *>(pool + s_to[k]) = x[i];
       }
     }
   }
 }
 
-// Few tasks: a task's rows over many workgroups. Each takes the next chunk of its (task, keys
-// or values) by a ticket, reads the chunk's rows into registers, says so, and writes them once
-// all chunks before it have said so: what it overwrites are rows of theirs or its own. A
-// chunk waits for earlier tickets only, whose workgroups are running and wait for nothing
-// before they say so; every wait ends.
-constexpr int kFewUnits = 8; // units of a lane
+// A stage's tokens in 16 bytes of one dim, a round of kMove * N pieces in the order of their
+// tokens: what a later round reads of a dim lies behind what this one writes of it.
+template <int EB>
+__device__ __forceinline__ void move_turned(uint8_t *pool, uint32_t dims, int64_t step,
+                                            uint32_t cnt, const int64_t *s_from,
+                                            const int64_t *s_to, const float *s_ratio) {
+  constexpr int N = EB == 4 ? 4 : 2;
+  constexpr uint32_t TOK = 16 / EB;
+  const uint32_t pieces = (cnt + TOK - 1u) / TOK * dims;
+  for (uint32_t p0 = 0; p0 < pieces; p0 += kMove * N) {
+    uint4 x[N];
+    bool moves[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t p = p0 + (uint32_t)i * kMove + threadIdx.x, pc = min(p, pieces - 1u);
+      moves[i] = gather16<EB>(pool + pc % dims * step, s_from, pc / dims * TOK, cnt, x[i]);
+      moves[i] = moves[i] && p < pieces;
+      gather_step<EB>(i, x);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      hold(x[i]);
+    asm volatile("s_barrier" ::: "memory");
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const uint32_t p = p0 + (uint32_t)i * kMove + threadIdx.x;
+      if (moves[i])
+        scatter16<EB>(pool + p % dims * step, s_to, s_ratio, p / dims * TOK, cnt, x[i]);
+    }
+  }
+}
 
-template <bool FP8>
-__global__ void __launch_bounds__(kMove) evict_move_few(EParams P, uint32_t units, uint32_t eb) {
-  constexpr uint32_t MOST = kMove / 4 * kFewUnits; // rows of a chunk (4 units a row at least)
+template <int EB>
+__global__ void __launch_bounds__(kMove, 4) evict_move(EParams P, Mode k_mode, Mode v_mode) {
+  typedef typename Elem<EB>::type E;
+  constexpr bool FP8 = EB == 1;
+  __shared__ int64_t s_from[kStage], s_to[kStage];
+  __shared__ float s_ratio[FP8 ? kStage : 1];
+  if (blockIdx.x >= P.row_groups) { // the wide selection's weights
+    move_weights(P, blockIdx.x - P.row_groups);
+    return;
+  }
+  const uint32_t task = blockIdx.x >> 1;
+  const bool vals = (blockIdx.x & 1u) != 0u;
+  const uint32_t r = task / P.Hkv, h = task % P.Hkv;
+  const Req q = req_of(P, r);
+  const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
+  if (q.m == q.n || q.m == 0u || kept[0] < 0)
+    return;
+  const Side S = side_of<EB>(P, task, h, vals);
+  const Mode mode = vals ? v_mode : k_mode;
+  for (uint32_t j0 = 0; j0 < q.m; j0 += kStage) {
+    const uint32_t cnt = min(kStage, q.m - j0);
+    __syncthreads(); // the previous stage's places have been used
+    places<FP8>(P, q, h, S, kept, j0, cnt, s_from, s_to, s_ratio);
+    __syncthreads();
+    if (mode == kRows)
+      move_units<uint4, 4, FP8>(S.pool, P.D * EB / 16u, 16, cnt, s_from, s_to, s_ratio);
+    else if (mode == kTurned)
+      move_turned<EB>(S.pool, P.D, S.dim, cnt, s_from, s_to, s_ratio);
+    else
+      move_units<E, 4, FP8>(S.pool, P.D, S.dim, cnt, s_from, s_to, s_ratio);
+  }
+}
+
+// Few tasks: a task's tokens over many workgroups. Each takes the next chunk of its (task, keys
+// or values) by a ticket, reads the chunk's tokens into registers, says so, and writes them
+// once all chunks before it have said so: what it overwrites are tokens of theirs or its own.
+// A chunk waits for earlier tickets only, whose workgroups are running and wait for nothing
+// before they say so; every wait ends.
+constexpr int kFewUnits = 8; // 16-byte units of a lane
+
+// Tokens of a chunk: a multiple of 16, so that a turned unit lies in one chunk.
+__host__ __device__ inline uint32_t few_rows(uint32_t units) {
+  return kMove / units * kFewUnits & ~15u;
+}
+
+template <int EB, bool TURNED>
+__global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
+  constexpr bool FP8 = EB == 1;
+  constexpr uint32_t MOST = kMove / 4 * kFewUnits; // tokens of a chunk (4 units each at least)
+  constexpr uint32_t TOK = 16 / EB;
   __shared__ int64_t s_from[MOST], s_to[MOST];
   __shared__ float s_ratio[FP8 ? MOST : 1];
   __shared__ uint32_t s_chunk;
@@ -794,36 +943,39 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P, uint32_t unit
   if (tid == 0)
     s_chunk = atomicAdd(ticket, 1u);
   __syncthreads();
-  const uint32_t rows = kMove / units, chunk = s_chunk, j0 = chunk * rows * kFewUnits;
+  const uint32_t units = P.D * EB / 16u, each = few_rows(units), chunk = s_chunk;
+  const uint32_t j0 = chunk * each;
   if (j0 >= q.m)
     return;
-  uint8_t *pool = vals ? P.v + (int64_t)h * P.vhs * eb : P.k + (int64_t)h * P.khs * eb;
-  const int64_t ps_b = (vals ? P.vps : P.kps) * eb, ts_b = (vals ? P.vts : P.kts) * eb;
-  const float *scale = vals ? P.vs : P.ks;
-  const float *ns = P.new_scale + ((int64_t)task * 2 + (vals ? 1 : 0)) * P.new_pages;
-  const uint32_t cnt = min(rows * kFewUnits, q.m - j0);
-  for (uint32_t i = tid; i < cnt; i += kMove) {
-    const uint32_t j = j0 + i, src = (uint32_t)kept[j];
-    const uint32_t sb = div_ps(P, src), db = div_ps(P, j);
-    const int64_t sp = P.bt[q.row + sb], dp = P.bt[q.row + db];
-    bool moves = src != j;
-    if constexpr (FP8) {
-      const float was = scale[(sp * P.Hkv + h) * P.scale_stride], now = ns[db];
-      s_ratio[i] = was != now ? was / now : -1.f; // below 0: the codes stay
-      moves = moves || was != now;
-    }
-    s_from[i] = moves ? sp * ps_b + (int64_t)(src - sb * P.ps) * ts_b : -1;
-    s_to[i] = dp * ps_b + (int64_t)(j - db * P.ps) * ts_b;
-  }
+  const uint32_t cnt = min(each, q.m - j0);
+  const Side S = side_of<EB>(P, task, h, vals);
+  places<FP8>(P, q, h, S, kept, j0, cnt, s_from, s_to, s_ratio);
   __syncthreads();
-  const uint32_t rr = tid / units, off = tid % units * 16u;
+  // turned: unit p is of dim p % D, of the tokens from p / D * TOK on
+  const bool turned = TURNED && vals;
+  const uint32_t most = (cnt + TOK - 1u) / TOK * P.D;
+  const uint32_t rows = kMove / units, rr = tid / units, off = tid % units * 16u;
   uint4 x[kFewUnits];
+  uint32_t moves = 0u;
+  if (!turned) {
 #pragma unroll
-  for (int i = 0; i < kFewUnits; ++i) {
-    const uint32_t k = (uint32_t)i * rows + rr;
-    x[i] = uint4{};
-    if (rr < rows && k < cnt && s_from[k] >= 0)
-      x[i] = *reinterpret_cast<const uint4 *>(pool + s_from[k] + off);
+    for (int i = 0; i < kFewUnits; ++i) {
+      const uint32_t k = (uint32_t)i * rows + rr;
+      x[i] = uint4{};
+      if (rr < rows && k < cnt && s_from[k] >= 0) {
+        moves |= 1u << i;
+        x[i] = *reinterpret_cast<const uint4 *>(S.pool + s_from[k] + off);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kFewUnits; ++i) {
+      const uint32_t p = (uint32_t)i * kMove + tid, pc = min(p, most - 1u);
+      const bool any =
+          gather16<EB>(S.pool + pc % P.D * S.dim, s_from, pc / P.D * TOK, cnt, x[i]);
+      moves |= any && p < most ? 1u << i : 0u;
+      gather_step<EB>(i, x);
+    }
   }
 #pragma unroll
   for (int i = 0; i < kFewUnits; ++i)
@@ -839,14 +991,19 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P, uint32_t unit
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kFewUnits; ++i) {
-    const uint32_t k = (uint32_t)i * rows + rr;
-    if (rr < rows && k < cnt && s_from[k] >= 0) {
+    if (!((moves >> i) & 1u))
+      continue;
+    if (turned) {
+      const uint32_t p = (uint32_t)i * kMove + tid;
+      scatter16<EB>(S.pool + p % P.D * S.dim, s_to, s_ratio, p / P.D * TOK, cnt, x[i]);
+    } else {
+      const uint32_t k = (uint32_t)i * rows + rr;
       if constexpr (FP8) {
         const float f = s_ratio[k];
         if (f >= 0.f)
           recode(x[i], f);
       }
-      *reinterpret_cast<uint4 *>(pool + s_to[k] + off) = x[i];
+      *reinterpret_cast<uint4 *>(S.pool + s_to[k] + off) = x[i];
     }
   }
 }
@@ -920,29 +1077,39 @@ uint64_t wide_bytes(const SchedEvictArgs *a) {
     return 0;
   return (uint64_t)a->num_requests * a->num_kv_heads * (3u * kWideBins + 1u + 2u * wide_chunks(a)) * 4u;
 }
-// Rows that evict_move_few moves: in 16-byte units, 4 to kMove of them.
-bool wide_rows(const SchedEvictArgs *a) {
-  const int64_t eb = elem_bytes(a->kv_dtype);
-  auto rows16 = [&](int64_t x) { return (x * eb) % 16 == 0; };
-  return a->v_dim_stride == 1 && (a->head_dim * eb) % 16 == 0 && (uintptr_t)a->k_pool % 16 == 0 &&
-         (uintptr_t)a->v_pool % 16 == 0 && rows16(a->k_page_stride) && rows16(a->k_head_stride) &&
-         rows16(a->k_tok_stride) && rows16(a->v_page_stride) && rows16(a->v_head_stride) &&
-         rows16(a->v_tok_stride);
+// Each tensor in 16-byte units where its strides allow. d-major, 8 kv-heads of 128 (us, V by
+// element / turned): 32 requests of 2048, half kept, 258 / 160; 2 of 2000 168 / 33; one of
+// 65537, an eighth kept, 1067 / 120.
+bool in16(const SchedEvictArgs *a, int64_t x) { return x * elem_bytes(a->kv_dtype) % 16 == 0; }
+Mode k_mode_of(const SchedEvictArgs *a) {
+  return in16(a, a->head_dim) && (uintptr_t)a->k_pool % 16 == 0 && in16(a, a->k_page_stride) &&
+                 in16(a, a->k_head_stride) && in16(a, a->k_tok_stride)
+             ? kRows
+             : kElems;
+}
+Mode v_mode_of(const SchedEvictArgs *a) {
+  if ((uintptr_t)a->v_pool % 16 || !in16(a, a->v_page_stride) || !in16(a, a->v_head_stride))
+    return kElems;
+  if (a->v_dim_stride == 1)
+    return in16(a, a->head_dim) && in16(a, a->v_tok_stride) ? kRows : kElems;
+  return in16(a, a->v_dim_stride) && in16(a, a->page_size) ? kTurned : kElems;
 }
 // Whether the rows are cut over workgroups. In us, with one workgroup per task and tensor
 // against chunks (head dim 128, bf16): 8 tasks of 1000 tokens 23.0 / 19.2, 192 of 1200 51.4 /
 // 48.8, 192 of 2048 fp8 47.7 / 44.9; at 256 tasks even (1200 tokens 62.1 / 62.8) or worse (2048
 // 77.7 / 81.9), and at 360 kept tokens and fewer too (8 of 300 12.9 / 13.2, 32 of 400 17.3 / 17.7).
+// d-major: 256 tasks of 2048 fp8 134 / 104, 512 of 1000 215 / 135; bf16 160 / 160, 1024 of
+// 1000 428 / 420.
 constexpr uint32_t kMoveFill = 512; // workgroups of evict_move that fill the card
+constexpr uint32_t kTurnFill = 4096;
 constexpr uint32_t kFewKeep = 512;
 bool few_applies(const SchedEvictArgs *a) {
-  return 2ull * a->num_requests * a->num_kv_heads < kMoveFill &&
+  return 2ull * a->num_requests * a->num_kv_heads < (a->v_dim_stride == 1 ? kMoveFill : kTurnFill) &&
          a->head_dim * elem_bytes(a->kv_dtype) >= 64u && a->max_keep > kFewKeep;
 }
 uint32_t few_chunks(const SchedEvictArgs *a) {
   const uint32_t units = a->head_dim * elem_bytes(a->kv_dtype) / 16u;
-  const uint32_t rows = kMove / units * kFewUnits;
-  return (a->max_keep + rows - 1u) / rows;
+  return (a->max_keep + few_rows(units) - 1u) / few_rows(units);
 }
 uint64_t move_bytes(const SchedEvictArgs *a) {
   if (!few_applies(a))
@@ -985,6 +1152,10 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   if (a->v_tok_stride != 1 && a->v_dim_stride != 1)
     return set_error(-1, "sched_kv_evict: V needs v_tok_stride == 1 (d-major) or v_dim_stride "
                          "== 1 (token-major)");
+  for (int64_t st : {a->k_page_stride, a->k_head_stride, a->k_tok_stride, a->v_page_stride,
+                     a->v_head_stride, a->v_tok_stride, a->v_dim_stride})
+    if (st < 0)
+      return set_error(-1, "sched_kv_evict: a pool's stride is negative");
   const uint32_t eb = elem_bytes(a->kv_dtype);
   if ((uintptr_t)a->k_pool % eb || (uintptr_t)a->v_pool % eb)
     return set_error(-1, "sched_kv_evict: a pool is not aligned to its elements");
@@ -1015,7 +1186,8 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   const uint32_t tasks = P.R * P.Hkv;
   const uint64_t longest = (uint64_t)a->max_pages * a->page_size;
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const bool many = wide_applies(a), few = few_applies(a) && wide_rows(a);
+  const Mode k_mode = k_mode_of(a), v_mode = v_mode_of(a);
+  const bool many = wide_applies(a), few = few_applies(a) && k_mode == kRows && v_mode != kElems;
   if (few) {
     P.moves = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->workspace) + scale_bytes(a) +
                                            wide_bytes(a));
@@ -1040,25 +1212,18 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   }
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a->max_keep > 0) {
-    const bool wide = wide_rows(a);
-    const uint32_t units = wide ? a->head_dim * eb / 16u : a->head_dim;
-    const int64_t k_step = wide ? 16 : eb, v_step = wide ? 16 : a->v_dim_stride * eb;
     P.row_groups = 2u * tasks * (few ? P.move_chunks : 1u);
     const dim3 grid(P.row_groups + (many ? tasks : 0u)), block(kMove);
-    if (few && fp8)
-      hipLaunchKernelGGL(evict_move_few<true>, grid, block, 0, s, P, units, eb);
-    else if (few)
-      hipLaunchKernelGGL(evict_move_few<false>, grid, block, 0, s, P, units, eb);
-    else if (wide && fp8)
-      hipLaunchKernelGGL((evict_move<uint4, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
-    else if (wide)
-      hipLaunchKernelGGL((evict_move<uint4, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
-    else if (fp8)
-      hipLaunchKernelGGL((evict_move<uint8_t, true>), grid, block, 0, s, P, units, k_step, v_step, eb);
-    else if (eb == 2)
-      hipLaunchKernelGGL((evict_move<uint16_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
-    else
-      hipLaunchKernelGGL((evict_move<uint32_t, false>), grid, block, 0, s, P, units, k_step, v_step, eb);
+    if (few) {
+      const bool turned = v_mode == kTurned;
+      auto fn = eb == 1   ? (turned ? evict_move_few<1, true> : evict_move_few<1, false>)
+                : eb == 2 ? (turned ? evict_move_few<2, true> : evict_move_few<2, false>)
+                          : (turned ? evict_move_few<4, true> : evict_move_few<4, false>);
+      hipLaunchKernelGGL(fn, grid, block, 0, s, P);
+    } else {
+      auto fn = eb == 1 ? evict_move<1> : eb == 2 ? evict_move<2> : evict_move<4>;
+      hipLaunchKernelGGL(fn, grid, block, 0, s, P, k_mode, v_mode);
+    }
     e = hipGetLastError();
     if (e == hipSuccess && fp8) {
       hipLaunchKernelGGL(evict_scales, dim3(tasks), dim3(256), 0, s, P);

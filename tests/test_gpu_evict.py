@@ -197,8 +197,25 @@ def test_wide_without_what_is_not_cut():
 
 @pytest.mark.parametrize("kv,d", [(torch.float32, 16), (torch.bfloat16, 32), (FP8, 64),
                                   (FP8, 256), (torch.float32, 256), (torch.float16, 96)])
-def test_rows_in_chunks(kv, d):
-    check([2000, 700, 3], [1900, 513, 2], kv=kv, d=d, hkv=2, recent=7)
+@pytest.mark.parametrize("layout", ["tokmajor", "dmajor"])
+def test_rows_in_chunks(kv, d, layout):
+    check([2000, 700, 3], [1900, 513, 2], kv=kv, d=d, hkv=2, recent=7, layout=layout)
+
+
+@pytest.mark.parametrize("kv", [torch.float32, torch.bfloat16, FP8])
+@pytest.mark.parametrize("ps,d", [(4, 20), (8, 64), (12, 64), (32, 128), (48, 256), (256, 64)])
+def test_turned_values(kv, ps, d):
+    """d-major values in pieces of 16 bytes where a page holds whole ones, else by
+    element; what is kept ends inside a piece."""
+    check([600, 9, 277, 0, 130], [301, 4, 276, 0, 129], kv=kv, ps=ps, d=d, layout="dmajor", sink=1,
+          recent=4)
+
+
+@pytest.mark.parametrize("kv", [torch.bfloat16, FP8])
+def test_turned_values_of_more_than_a_stage(kv):
+    """Beyond the places that are held at a time, with and without chunks."""
+    check([5000, 40], [4100, 30], kv=kv, d=64, layout="dmajor", hkv=1)
+    check([3000] + [20] * 259, [2999] + [7] * 259, kv=kv, d=32, layout="dmajor", hkv=1)
 
 
 def test_another_stream_and_few_rows_in_a_graph():
