@@ -182,9 +182,10 @@ typedef struct SchedRotaryArgs {
   void *k_pool, *v_pool;
   int64_t kp_page_stride, kp_head_stride, kp_tok_stride; /* elements, dims contiguous */
   int64_t vp_page_stride, vp_head_stride, vp_tok_stride;
+  int64_t vp_dim_stride;  /* 1: token-major V; vp_tok_stride 1: d-major */
 } SchedRotaryArgs;
 
-/* Fill *a with defaults (ABI version, BF16 rows, F32 weights, eps 1e-6). */
+/* Fill *a with defaults (ABI version, BF16 rows, F32 weights, eps 1e-6, vp_dim_stride 1). */
 void sched_rotary_default_args(SchedRotaryArgs *a);
 
 /* Run it on `stream`, one launch. Returns 0, or -1 with sched_pd_last_error() set. */

@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "common.h"
 #include "rt_internal.h"
@@ -40,11 +41,12 @@ struct RParams {
   int64_t cs_stride;
   uint32_t *errors;
   uint32_t T, Hq, Hkv, d, rot, max_pos;
+  uint32_t v_rows; // value rows that go along with a token's keys
   uint32_t w_dtype, inter, pos64;
   float eps;
   // the cache (kp == nullptr: none)
   void *kp, *vp;
-  int64_t kps, khs, kts, vps, vhs, vts;
+  int64_t kps, khs, kts, vps, vhs, vts, vds;
   const int32_t *app, *ctx, *table, *pind;
   uint32_t ps, bt_stride;
   uint64_t num_pages;
@@ -137,7 +139,7 @@ template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams 
   const uint32_t lane = threadIdx.x & 63u;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const Span S = span_of(P, blockIdx.x);
-  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), half = P.rot / 2u;
+  const uint32_t rows = P.Hq + P.Hkv + P.v_rows, half = P.rot / 2u;
   for (int64_t i = blockIdx.y; i < S.n; i += gridDim.y) {
     const int64_t tok = S.a0 + i;
     const int64_t pos = position_of(P, tok);
@@ -161,7 +163,7 @@ template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams 
                          : isv ? tok * P.v_ts + h * P.v_hs
                                : tok * P.k_ts + h * P.k_hs;
       void *dst;
-      int64_t d0;
+      int64_t d0, ds = 1;
       if (isq) {
         dst = P.qo, d0 = tok * P.qo_ts + h * P.qo_hs;
       } else if (P.kp == nullptr) {
@@ -169,7 +171,7 @@ template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams 
       } else if (at.page < 0) {
         continue;
       } else if (isv) {
-        dst = P.vp, d0 = at.page * P.vps + h * P.vhs + at.slot * P.vts;
+        dst = P.vp, d0 = at.page * P.vps + h * P.vhs + at.slot * P.vts, ds = P.vds;
       } else {
         dst = P.kp, d0 = at.page * P.kps + h * P.khs + at.slot * P.kts;
       }
@@ -204,7 +206,7 @@ template <int DT> __global__ void __launch_bounds__(kBlock) rotary_rows(RParams 
           const float b = w != nullptr ? y[u] * (inv * load_w(P, w, p)) : y[u];
           o = first ? o * c - b * s : o * c + b * s;
         }
-        st<DT>(dst, d0 + e, o);
+        st<DT>(dst, d0 + e * ds, o);
       }
     }
   }
@@ -310,6 +312,31 @@ struct Deal {
   float inv_d;
 };
 
+// A lane group's tokens of a d-major V head: the lane's 16 bytes of a row go to as many rows
+// as they have elements.
+template <int EB>
+__device__ __forceinline__ void values_apart(const RParams &P, const Span &S, const Deal &D,
+                                             uint32_t h, uint32_t d0, uint32_t tsub, int64_t step) {
+  typedef typename std::conditional<EB == 4, uint32_t, uint16_t>::type E;
+  for (int64_t base = (int64_t)blockIdx.y * step; base < S.n; base += (int64_t)gridDim.y * step) {
+    for (uint32_t k = 0; k < D.per; ++k) {
+      const int64_t i = base + tsub + (int64_t)k * D.ts;
+      if (i >= S.n)
+        break;
+      const int64_t pos = position_of(P, S.a0 + i);
+      const u32x4_t x = *reinterpret_cast<const u32x4_t *>(
+          static_cast<const char *>(P.v) + ((S.a0 + i) * P.v_ts + (int64_t)h * P.v_hs + d0) * EB);
+      const Place at = place_of(P, S, i);
+      if ((uint64_t)pos >= (uint64_t)P.max_pos || at.page < 0)
+        continue;
+      E *to = static_cast<E *>(P.vp) + at.page * P.vps + (int64_t)h * P.vhs + at.slot + d0 * P.vds;
+#pragma unroll
+      for (int e = 0; e < 16 / EB; ++e)
+        to[e * P.vds] = (E)(x[e * EB / 4] >> (8 * (e * EB % 4)));
+    }
+  }
+}
+
 // Rows that 16-byte loads reach: 2^LG lanes hold a row (V elements each), so a wave holds
 // 64 >> LG rows; the sum of squares and the exchange of the pairs' halves (HLG: lanes whose
 // numbers differ in that bit hold them; -1: neighbouring pairs, within a lane) stay within
@@ -324,7 +351,7 @@ __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
   constexpr int NC = INTER ? V / 2 : V;         // angles of a lane
   constexpr uint32_t L = 1u << LG;
   const uint32_t tid = threadIdx.x, li = tid & (L - 1u);
-  const uint32_t rows = P.Hq + P.Hkv + (P.kp ? P.Hkv : 0u), half = P.rot / 2u, d0 = li * V;
+  const uint32_t rows = P.Hq + P.Hkv + P.v_rows, half = P.rot / 2u, d0 = li * V;
   const uint32_t f = blockIdx.z * (kBlock >> LG) + (tid >> LG);
   const uint32_t tsub = f / rows, row = f - tsub * rows;
   const Span S = span_of(P, blockIdx.x);
@@ -337,6 +364,11 @@ __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
   const bool paged = !isq && P.kp != nullptr;
   const bool turned = !isv && d0 < P.rot, first = INTER || d0 < half;
   const void *w = isv ? nullptr : isq ? P.qw : P.kw;
+  if (isv && P.vds != 1) {
+    if (live)
+      values_apart<EB>(P, S, D, h, d0, tsub, step);
+    return; // (exchanges stay within a row's lanes)
+  }
   float wt[V];
 #pragma unroll
   for (int e = 0; e < V; ++e)
@@ -455,6 +487,68 @@ __global__ void __launch_bounds__(kBlock) rotary_vec(RParams P, Deal D) {
   }
 }
 
+// The values of many tokens into a d-major cache: a tile of positions through LDS, read by
+// rows and written in 16 bytes of a dim where all of its tokens go there. 8 prompts of up to
+// 3000 tokens, 32 / 8 heads of 128 bf16, with the norm and rotation: 163 us; the values by
+// element among the other rows 272; into a token-major cache 151.
+template <int EB> __global__ void __launch_bounds__(kBlock) values_turned(RParams P) {
+  typedef typename std::conditional<EB == 4, uint32_t, uint16_t>::type E;
+  constexpr uint32_t TT = 128 / EB, TOK = 16 / EB, NG = TT / TOK;
+  __shared__ __attribute__((aligned(4))) E s_row[TT][256 + 4 / EB];
+  __shared__ int64_t s_to[TT];
+  const uint32_t tid = threadIdx.x, h = blockIdx.z, units = P.d / TOK;
+  const Span S = span_of(P, blockIdx.x);
+  const int64_t start = S.ctx - S.n, lowest = start > 0 ? start / TT * TT : 0;
+  const char *src = static_cast<const char *>(P.v) + (int64_t)h * P.v_hs * EB;
+  char *dst = static_cast<char *>(P.vp) + (int64_t)h * P.vhs * EB;
+  for (int64_t t0 = lowest + (int64_t)blockIdx.y * TT; t0 < S.ctx; t0 += (int64_t)gridDim.y * TT) {
+    __syncthreads(); // the last tile's have been written
+    if (tid < TT) {
+      const int64_t i = t0 + tid - start;
+      int64_t to = -1;
+      if (i >= 0 && i < S.n) {
+        const int64_t pos = position_of(P, S.a0 + i);
+        const Place at = place_of(P, S, i);
+        if ((uint64_t)pos < (uint64_t)P.max_pos && at.page >= 0)
+          to = at.page * P.vps + at.slot;
+      }
+      s_to[tid] = to;
+    }
+    for (uint32_t u = tid; u < TT * units; u += kBlock) {
+      const uint32_t k = u / units, c = u - k * units;
+      const int64_t i = t0 + k - start;
+      if (i >= 0 && i < S.n) {
+        const char *from = src + (S.a0 + i) * P.v_ts * EB + 16u * c;
+        const u32x4_t x = *reinterpret_cast<const u32x4_t *>(from);
+        uint32_t *to = reinterpret_cast<uint32_t *>(&s_row[k][c * TOK]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          to[w] = x[w];
+      }
+    }
+    __syncthreads();
+    for (uint32_t p = tid; p < NG * P.d; p += kBlock) {
+      const uint32_t k0 = p % NG * TOK, e = p / NG;
+      char *row = dst + (int64_t)e * P.vds * EB;
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      bool all = true;
+#pragma unroll
+      for (uint32_t t = 0; t < TOK; ++t) {
+        all = all && s_to[k0 + t] >= 0;
+        w[t * EB / 4] |= (uint32_t)s_row[k0 + t][e] << (8 * (t * EB % 4));
+      }
+      if (all) {
+        *reinterpret_cast<u32x4_t *>(row + s_to[k0] * EB) = u32x4_t{w[0], w[1], w[2], w[3]};
+      } else {
+#pragma unroll
+        for (uint32_t t = 0; t < TOK; ++t)
+          if (s_to[k0 + t] >= 0)
+            *reinterpret_cast<E *>(row + s_to[k0 + t] * EB) = s_row[k0 + t][e];
+      }
+    }
+  }
+}
+
 typedef void (*VecFn)(RParams, Deal);
 
 // A row's lanes (log2) and the lane bit that pairs' halves differ in (-1: none): full,
@@ -520,6 +614,7 @@ void sched_rotary_default_args(SchedRotaryArgs *a) {
   a->dtype = SCHED_PD_BF16;
   a->w_dtype = SCHED_PD_F32;
   a->eps = 1e-6f;
+  a->vp_dim_stride = 1;
 }
 
 int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
@@ -564,6 +659,9 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
                        (unsigned long long)a->num_pages);
     if (!a->page_indptr && a->bt_stride == 0)
       return set_error(-1, "sched_qk_norm_rope: bt_stride is 0 with a 2-D block table");
+    if (a->vp_tok_stride != 1 && a->vp_dim_stride != 1)
+      return set_error(-1, "sched_qk_norm_rope: V needs vp_tok_stride == 1 (d-major) or "
+                           "vp_dim_stride == 1 (token-major)");
   }
   const uint32_t es = esize(a->dtype);
   for (const void *p : {a->q, a->k, a->v, (const void *)a->q_out, (const void *)a->k_out,
@@ -590,6 +688,7 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
     P.kp = a->k_pool, P.vp = a->v_pool;
     P.kps = a->kp_page_stride, P.khs = a->kp_head_stride, P.kts = a->kp_tok_stride;
     P.vps = a->vp_page_stride, P.vhs = a->vp_head_stride, P.vts = a->vp_tok_stride;
+    P.vds = a->vp_dim_stride;
     P.app = a->append_indptr, P.ctx = a->ctx_lens, P.table = a->block_table;
     P.pind = a->page_indptr, P.ps = a->page_size, P.bt_stride = a->bt_stride;
     P.num_pages = a->num_pages;
@@ -609,21 +708,30 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
              pieces(P.k_ts) && pieces(P.k_hs) && pieces(P.qo_ts) && pieces(P.qo_hs);
   if (cache)
     vec = vec && pieces(P.v_ts) && pieces(P.v_hs) && pieces(P.kps) && pieces(P.khs) &&
-          pieces(P.kts) && pieces(P.vps) && pieces(P.vhs) && pieces(P.vts);
+          pieces(P.kts) &&
+          (P.vds != 1 || (pieces(P.vps) && pieces(P.vhs) && pieces(P.vts)));
   else
     vec = vec && pieces(P.ko_ts) && pieces(P.ko_hs);
   for (const void *p : {a->q, a->k, cache ? a->v : nullptr, (const void *)a->q_out,
                         cache ? nullptr : (const void *)a->k_out, (const void *)a->k_pool,
-                        (const void *)(cache ? a->v_pool : nullptr)})
+                        (const void *)(cache && P.vds == 1 ? a->v_pool : nullptr)})
     vec = vec && (uintptr_t)p % 16 == 0;
   for (const void *p : {a->q_weight, a->k_weight})
     vec = vec && (uintptr_t)p % (a->w_dtype == SCHED_PD_F32 ? 16 : 8) == 0;
   VecFn fn = nullptr;
   Deal D{1u, 1u, 1.f / (float)a->head_dim};
+  bool turn = false;
+  P.v_rows = cache ? P.Hkv : 0u;
   if (vec) {
-    const uint32_t rows = P.Hq + P.Hkv + (cache ? P.Hkv : 0u);
+    uint32_t rows = P.Hq + P.Hkv + P.v_rows;
     const uint32_t groups = kBlock / (a->head_dim / v);
     auto across = [&](uint32_t t) { return (t * rows + groups - 1u) / groups; };
+    // many tokens' values into a d-major cache: a launch of their own
+    turn = cache && P.vds != 1 && P.ps % v == 0 && pieces(P.vps) && pieces(P.vhs) &&
+           pieces(P.vds) && (uintptr_t)a->v_pool % 16 == 0 &&
+           (uint64_t)P.T * across(1) >= kOneToken;
+    if (turn)
+      P.v_rows = 0u, rows -= P.Hkv;
     // as many tokens side by side, at most 8, as leave the fewest lane groups idle
     uint32_t ts = 1, best = ~0u;
     for (uint32_t t = 1; t <= 8; ++t) {
@@ -649,7 +757,14 @@ int sched_qk_norm_rope(const SchedRotaryArgs *a, void *stream) {
   }
   if (fn) {
     hipLaunchKernelGGL(fn, grid, dim3(kBlock), 0, s, P, D);
+    if (turn) {
+      const uint32_t tiles = (most + 128u / es - 1u) / (128u / es) + 1u;
+      const dim3 over(a->num_requests, tiles < 65535u ? tiles : 65535u, P.Hkv);
+      hipLaunchKernelGGL(es == 4 ? values_turned<4> : values_turned<2>, over, dim3(kBlock), 0, s,
+                         P);
+    }
   } else {
+    P.v_rows = cache ? P.Hkv : 0u;
     auto every = a->dtype == SCHED_PD_F32    ? rotary_rows<SCHED_PD_F32>
                  : a->dtype == SCHED_PD_BF16 ? rotary_rows<SCHED_PD_BF16>
                                              : rotary_rows<SCHED_PD_F16>;

@@ -34,7 +34,7 @@ def cos_sin_table(max_pos: int, rot_dim: int, base: float = 10000.0, device="cud
     return torch.cat([ang.cos(), ang.sin()], 1).float().to(device)
 
 
-_ROWS = (0,) * 17        # the block's cache fields without a cache
+_ROWS = (0,) * 18        # the block's cache fields without a cache
 
 
 def _call(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, k_out, errors,
@@ -138,11 +138,14 @@ def append_rotated(q, k, v, positions, cos_sin, append_indptr, ctx_lens, k_pool,
     ctx_lens[r]-1 of its pages (ctx_lens counts tokens after the append; `positions` are
     the rotation's and need not follow them: after an eviction they do not).
 
-    One launch into a cache of the rows' type with token-major V; other caches (fp8,
-    d-major V, another type) take qk_norm_rope() and kv_cache.append(), the keys rounded to
-    the rows' type in between. `errors` counts tokens with a position outside cos_sin
-    and (token, kv-head) pairs that have no place in the cache."""
-    if k_pool.dtype != q.dtype or v_layout != "tokmajor" or k_pool.dim() != 4:
+    One launch into a cache of the rows' type (two where many tokens go to a d-major V);
+    other caches (fp8, another type) take qk_norm_rope() and kv_cache.append(), the keys
+    rounded to the rows' type in between, and that writer's zeros behind the last value of
+    a d-major V. `errors` counts tokens with a position outside cos_sin and (token,
+    kv-head) pairs that have no place in the cache."""
+    if v_layout not in ("tokmajor", "dmajor"):
+        raise ValueError(f"v_layout must be 'dmajor' or 'tokmajor', got {v_layout!r}")
+    if k_pool.dtype != q.dtype or k_pool.dim() != 4:
         q_out, k_rot = qk_norm_rope(q, k, positions, cos_sin, q_weight=q_weight, k_weight=k_weight,
                                     eps=eps, interleaved=interleaved, q_out=q_out, errors=errors)
         kv_cache.append(k_rot, v.contiguous(), append_indptr, ctx_lens, k_pool, v_pool,
@@ -150,14 +153,16 @@ def append_rotated(q, k, v, positions, cos_sin, append_indptr, ctx_lens, k_pool,
                         v_scale=v_scale, max_append=max_append, errors=errors)
         return q_out
     P, hkv, ps, d = k_pool.shape
-    if v_pool.dtype != k_pool.dtype or v_pool.shape != k_pool.shape:
-        raise ValueError(f"token-major v_pool must be {k_pool.dtype} {tuple(k_pool.shape)}, got "
+    dm = v_layout == "dmajor"
+    if v_pool.dtype != k_pool.dtype or v_pool.shape != ((P, hkv, d, ps) if dm else k_pool.shape):
+        raise ValueError(f"{v_layout} v_pool must be {k_pool.dtype} "
+                         f"{(P, hkv, d, ps) if dm else tuple(k_pool.shape)}, got "
                          f"{v_pool.dtype} {tuple(v_pool.shape)}")
     if k.shape[1:] != (hkv, d):
         raise ValueError(f"k {tuple(k.shape)} vs pool heads/dims ({hkv}, {d})")
     ks, vs = k_pool.stride(), v_pool.stride()
     if ks[3] != 1 or vs[3] != 1:
-        raise ValueError("pool dims must be contiguous")
+        raise ValueError("pool dims must be contiguous (d-major V: tokens)")
     R = ctx_lens.numel()
     stride, _, indptr = table_of(R, block_table, page_indptr, ctx_lens)
     if append_indptr.dtype != torch.int32 or not append_indptr.is_contiguous() \
@@ -172,4 +177,5 @@ def append_rotated(q, k, v, positions, cos_sin, append_indptr, ctx_lens, k_pool,
     return _call(q, k, v, positions, cos_sin, q_weight, k_weight, eps, interleaved, q_out, None,
                  errors, (R, ps, stride, int(max_append), P, append_indptr.data_ptr(),
                           ctx_lens.data_ptr(), block_table.data_ptr(), indptr, k_pool.data_ptr(),
-                          v_pool.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1], vs[2]))
+                          v_pool.data_ptr(), ks[0], ks[1], ks[2], vs[0], vs[1],
+                          1 if dm else vs[2], vs[2] if dm else 1))

@@ -169,6 +169,7 @@ class SchedRotaryArgs(ctypes.Structure):
         ("k_pool", _p), ("v_pool", _p),
         ("kp_page_stride", _i64), ("kp_head_stride", _i64), ("kp_tok_stride", _i64),
         ("vp_page_stride", _i64), ("vp_head_stride", _i64), ("vp_tok_stride", _i64),
+        ("vp_dim_stride", _i64),
     ]
 
 
@@ -198,7 +199,7 @@ def default_maps_args() -> SchedMapsArgs:
 
 def default_rotary_args() -> SchedRotaryArgs:
     """Same defaults as sched_rotary_default_args() in C."""
-    return SchedRotaryArgs(abi_version=ROTARY_ABI_VERSION, dtype=BF16, w_dtype=F32, eps=1e-6)
+    return SchedRotaryArgs(abi_version=ROTARY_ABI_VERSION, dtype=BF16, w_dtype=F32, eps=1e-6, vp_dim_stride=1)
 
 
 def default_evict_args() -> SchedEvictArgs:

@@ -226,6 +226,41 @@ def test_append_matches_the_writer(dt, layout, counts, held):
         assert torch.equal(a.k_scale, b.k_scale) and torch.equal(a.v_scale, b.v_scale)
 
 
+@pytest.mark.parametrize("dt", TYPES)
+@pytest.mark.parametrize("layout", ["tokmajor", "dmajor"])
+@pytest.mark.parametrize("T,held", [(7, 9), (5000, 13)])
+@pytest.mark.parametrize("d,ps", [(128, 16), (96, 7)])
+def test_append_leaves_the_other_slots(dt, layout, T, held, d, ps):
+    """Slots behind the last token, before the first and of other pages keep their bytes."""
+    hq, hkv = 4, 2
+    n = -(-(held + T) // ps)
+    g = torch.Generator().manual_seed(T)
+    qkv, qw, kw = case(T, hq, hkv, d, dt, 13)
+    kp = torch.randn(n + 2, hkv, ps, d, generator=g).to(dt)
+    vp = torch.randn(*((n + 2, hkv, d, ps) if layout == "dmajor" else kp.shape),
+                     generator=g).to(dt)
+    pages = torch.randperm(n + 2, generator=g)[:n]
+    x, kd, vd = qkv.cuda(), kp.cuda(), vp.cuda()
+    table = rotary.cos_sin_table(8192, d)
+    pos = torch.arange(T) + held
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    q = rotary.append_rotated(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pos.cuda(), table,
+                              i32([0, T]), i32([held + T]), kd, vd, pages.int()[None].cuda(),
+                              v_layout=layout, q_weight=cu(qw), k_weight=cu(kw), errors=err)
+    rq, rk = rotary.qk_norm_rope(x[:, :hq], x[:, hq:hq + hkv], pos.cuda(), table, q_weight=cu(qw),
+                                 k_weight=cu(kw))
+    at = torch.arange(held, held + T)
+    p, s = pages[at // ps], at % ps
+    kp[p, :, s] = rk.cpu()
+    if layout == "dmajor":
+        vp[p, :, :, s] = qkv[:, hq + hkv:]
+    else:
+        vp[p, :, s] = qkv[:, hq + hkv:]
+    assert int(err) == 0 and torch.equal(q, rq)
+    assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+
+
 def test_append_without_a_place_is_counted():
     hq, hkv, d, ps = 2, 3, 64, 16
     qkv, qw, kw = case(20, hq, hkv, d, torch.bfloat16, 10)

@@ -111,6 +111,7 @@ def rotary_args(**kw):
     (dict(v=None), "a cache needs"), (dict(append_indptr=None), "a cache needs"),
     (dict(page_size=0), "page_size"), (dict(num_pages=0), "num_pages"), (dict(bt_stride=0), "bt_stride"),
     (dict(k=ctypes.c_void_p(0x10001)), "aligned"), (dict(num_tokens=1 << 31), "num_tokens"),
+    (dict(vp_dim_stride=16, vp_tok_stride=2), "V needs"),
 ])
 def test_rotary_refusals(schedlib, kw, msg):
     assert schedlib.sched_qk_norm_rope(ctypes.byref(rotary_args(**kw)), None) != 0
@@ -137,7 +138,7 @@ def evict_args(**kw):
     (dict(num_pages=0), "num_pages"), (dict(max_keep=1 << 31), "max_keep"),
     (dict(max_pages=1 << 21, bt_stride=1 << 21), "2^24 tokens"),
     (dict(weights=None), "required"), (dict(kept=None), "required"), (dict(bt_stride=3), "bt_stride"),
-    (dict(v_dim_stride=2), "V needs"), (dict(k_pool=ctypes.c_void_p(0x10001)), "aligned"),
+    (dict(v_dim_stride=2), "V needs"), (dict(k_page_stride=-64), "negative"), (dict(k_pool=ctypes.c_void_p(0x10001)), "aligned"),
     (dict(kv_dtype=abi.FP8_E4M3), "k_scale"),
     (dict(kv_dtype=abi.FP8_E4M3, k_scale=PTR, v_scale=PTR, workspace=None), "workspace"),
     (dict(kv_dtype=abi.FP8_E4M3, k_scale=PTR, v_scale=PTR, workspace_bytes=8), "workspace"),
