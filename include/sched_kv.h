@@ -222,7 +222,7 @@ typedef struct SchedEvictArgs {
   uint32_t head_dim;      /* multiple of 4, <= 256 */
   uint32_t page_size;     /* multiple of 4, <= 256 */
   uint32_t bt_stride;
-  uint32_t max_pages;     /* table width (2-D), or the page list's length */
+  uint32_t max_pages;     /* table width (2-D), or the page list's length; of at most 2^24 tokens */
   uint32_t max_keep;
   uint32_t sink, recent;
   uint32_t _pad0;

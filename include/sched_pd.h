@@ -457,7 +457,7 @@ typedef struct SchedMapsArgs {
   uint32_t page_size;    /* multiple of 16, at most 256 */
   uint32_t bt_stride;
   uint32_t max_pages;    /* table width, or the page list's length with page_indptr: a
-                            request's pages past it are not read */
+                            request's pages past it are not read. At most 2^24 tokens */
   uint32_t flags;        /* SCHED_PD_FLAG_FORCE_VALU or 0 */
   float sm_scale;        /* 0 = the default above */
   float decay;           /* WEIGHTED */

@@ -625,7 +625,8 @@ int sched_decode_maps(const SchedMapsArgs *a, void *stream) {
                  1.4426950408889634f;
   P.w = a->weights, P.w_ps = a->w_page_stride, P.w_hs = a->w_head_stride;
   P.counted = a->counted, P.decay = a->decay;
-  P.w_vec = ((uintptr_t)a->weights & 15u) == 0 && a->w_page_stride % 4 == 0 && a->w_head_stride % 4 == 0;
+  P.w_vec = ((uintptr_t)a->weights & 15u) == 0 && a->w_page_stride % 4 == 0 &&
+            a->w_head_stride % 4 == 0;
   P.lam = a->lam, P.nw = a->norm_weight, P.eps = a->eps, P.mul = a->out_scale;
   uint8_t *ws = static_cast<uint8_t *>(a->workspace);
   P.scores = reinterpret_cast<float *>(ws), P.score_blocks = plan.score_blocks;

@@ -822,7 +822,7 @@ __device__ __forceinline__ void move_units(uint8_t *pool, uint32_t units, int64_
       x[i] = nx[i];
     if (k0 + round < cnt)
       fetch(k0 + round);
-    // this round's rows are in registers on every lane before any of them is written: each
+    // the round's rows are in registers on every lane before any of them is written: each
     // lane waits for its own here (the next round's stay under way), then the barrier
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -1051,8 +1051,12 @@ int check_shape(const SchedEvictArgs *a) {
   return 0;
 }
 
+// The most tokens that a request of the call keeps: not more than its table holds.
+uint32_t most_kept(const SchedEvictArgs *a) {
+  return (uint32_t)std::min<uint64_t>(a->max_keep, (uint64_t)a->max_pages * a->page_size);
+}
 uint32_t new_pages_of(const SchedEvictArgs *a) {
-  return (uint32_t)(((uint64_t)a->max_keep + a->page_size - 1u) / a->page_size);
+  return (uint32_t)(((uint64_t)most_kept(a) + a->page_size - 1u) / a->page_size);
 }
 
 // Tables that reach past one workgroup's registers (evict_select<512, 24>'s 12288 tokens),
@@ -1070,12 +1074,14 @@ uint32_t wide_chunks(const SchedEvictArgs *a) {
 uint64_t scale_bytes(const SchedEvictArgs *a) {
   if (a->kv_dtype != SCHED_PD_FP8_E4M3)
     return 0;
-  return ((uint64_t)a->num_requests * a->num_kv_heads * 2u * new_pages_of(a) * 4u + 255u) / 256u * 256u;
+  const uint64_t tasks = (uint64_t)a->num_requests * a->num_kv_heads;
+  return (tasks * 2u * new_pages_of(a) * 4u + 255u) / 256u * 256u;
 }
 uint64_t wide_bytes(const SchedEvictArgs *a) {
   if (!wide_applies(a))
     return 0;
-  return (uint64_t)a->num_requests * a->num_kv_heads * (3u * kWideBins + 1u + 2u * wide_chunks(a)) * 4u;
+  const uint64_t tasks = (uint64_t)a->num_requests * a->num_kv_heads;
+  return tasks * (3u * kWideBins + 1u + 2u * wide_chunks(a)) * 4u;
 }
 // Each tensor in 16-byte units where its strides allow. d-major, 8 kv-heads of 128 (us, V by
 // element / turned): 32 requests of 2048, half kept, 258 / 160; 2 of 2000 168 / 33; one of
@@ -1104,12 +1110,13 @@ constexpr uint32_t kMoveFill = 512; // workgroups of evict_move that fill the ca
 constexpr uint32_t kTurnFill = 4096;
 constexpr uint32_t kFewKeep = 512;
 bool few_applies(const SchedEvictArgs *a) {
-  return 2ull * a->num_requests * a->num_kv_heads < (a->v_dim_stride == 1 ? kMoveFill : kTurnFill) &&
-         a->head_dim * elem_bytes(a->kv_dtype) >= 64u && a->max_keep > kFewKeep;
+  const uint32_t fill = a->v_dim_stride == 1 ? kMoveFill : kTurnFill;
+  return 2ull * a->num_requests * a->num_kv_heads < fill &&
+         a->head_dim * elem_bytes(a->kv_dtype) >= 64u && most_kept(a) > kFewKeep;
 }
 uint32_t few_chunks(const SchedEvictArgs *a) {
   const uint32_t units = a->head_dim * elem_bytes(a->kv_dtype) / 16u;
-  return (a->max_keep + few_rows(units) - 1u) / few_rows(units);
+  return (most_kept(a) + few_rows(units) - 1u) / few_rows(units);
 }
 uint64_t move_bytes(const SchedEvictArgs *a) {
   if (!few_applies(a))
@@ -1203,8 +1210,8 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
     hipLaunchKernelGGL(wide_count, grid, dim3(kWide), 0, s, P);
     hipLaunchKernelGGL(wide_keep, grid, dim3(kWide), 0, s, P);
     if (fp8)
-      hipLaunchKernelGGL(wide_scales, dim3(tasks, std::max(1u, (a->max_keep + 767u) / 768u)), dim3(1024), 0,
-                         s, P); // (a round has 769 tokens or more)
+      hipLaunchKernelGGL(wide_scales, dim3(tasks, std::max(1u, (most_kept(a) + 767u) / 768u)),
+                         dim3(1024), 0, s, P); // (a round has 769 tokens or more)
   } else if (longest <= kShort) {
     hipLaunchKernelGGL((evict_select<256, 16>), dim3(tasks), dim3(256), 0, s, P);
   } else {

@@ -67,6 +67,9 @@ def evict(k_pool, v_pool, weights, block_table, ctx_lens, keep_lens, *, sink=0, 
         raise ValueError(f"keep_lens must be contiguous int32 [{R}]")
     stride, pages, indptr = table_of(R, block_table, page_indptr, ctx_lens)
     max_keep = pages * ps if max_keep is None else int(max_keep)
+    if not 0 <= max_keep < 1 << 31:
+        raise ValueError(f"max_keep {max_keep}")
+    sink, recent = min(int(sink), (1 << 31) - 1), min(int(recent), (1 << 31) - 1)
     if kept is None:
         kept = torch.empty(R, hkv, max_keep, dtype=torch.int32, device=k_pool.device)
     elif kept.dtype != torch.int32 or kept.shape != (R, hkv, max_keep) or not kept.is_contiguous():

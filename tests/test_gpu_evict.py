@@ -2,6 +2,7 @@
 keys and values against the definition, bit for bit; ties, NaN, infinities and
 negative weights; every cache type and layout; what is not touched; and the serving
 steps together: rotated append, weighted decode, eviction, and on."""
+import ctypes
 import math
 
 import pytest
@@ -9,6 +10,7 @@ import torch
 
 import eviction
 import kv_cache
+import sched_abi as abi
 import maps_ref as mr
 import rotary
 
@@ -152,6 +154,19 @@ def test_page_list_and_separate_weights(kv):
 def test_max_keep_bounds_what_is_kept():
     check([300, 64], [200, 64], max_keep=50, recent=10)
     check([300, 64], [200, 300], max_keep=400)
+
+
+def test_bounds_beyond_any_table():
+    """max_keep, sink and recent past what tables hold; the outputs are what they size."""
+    check([300, 64], [200, 300], max_keep=5000, sink=1 << 40, recent=10)
+    check([300, 64], [200, 30], max_keep=100000, recent=1 << 40, kv=FP8)
+    a = abi.default_evict_args()
+    a.num_requests, a.num_kv_heads, a.head_dim, a.page_size = 100, 2, 128, 16
+    a.num_pages, a.max_pages, a.k_tok_stride, a.v_dim_stride = 1000, 40, 128, 1
+    a.max_keep = 640
+    need = abi.load_library().sched_kv_evict_workspace_bytes(ctypes.byref(a))
+    a.max_keep = (1 << 31) - 1
+    assert abi.load_library().sched_kv_evict_workspace_bytes(ctypes.byref(a)) == need > 0
 
 
 def test_nothing_to_cut():
