@@ -262,6 +262,41 @@ def test_another_stream_and_few_rows_in_a_graph():
         assert torch.equal(bits(a["k"]), bits(b["k"])) and torch.equal(bits(a["v"]), bits(b["v"]))
 
 
+def test_a_capture_without_a_pool_needs_a_workspace():
+    """What such a capture allocated would be freed under its graph: refused, and with a
+    workspace that the caller keeps, captured and replayed."""
+    hip = ctypes.CDLL("libamdhip64.so")
+    c = mr.paged([900, 40], 2, 64, 16, torch.bfloat16, seed=9)
+    w = weights_of(c, 2, 16, 9, "long")
+    kt = torch.tensor([700, 30], dtype=torch.int32).cuda()
+    ref = expected(c, w, w, [700, 30], 0, 0, 700)
+    x, wg = mr.to_gpu(c), w.cuda()
+    kept = torch.empty(2, 2, 700, dtype=torch.int32, device="cuda")
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+
+    def cut(**kw):
+        eviction.evict(x["k"], x["v"], wg, x["bt"], x["ctx"], kt, max_keep=700, kept=kept,
+                       v_layout="tokmajor", **kw)
+
+    side = torch.cuda.Stream()
+    graph, exe = ctypes.c_void_p(), ctypes.c_void_p()
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        h = ctypes.c_void_p(side.cuda_stream)
+        assert hip.hipStreamBeginCapture(h, 1) == 0         # thread-local mode
+        with pytest.raises(RuntimeError, match="workspace"):
+            cut()
+        cut(workspace=ws)
+        assert hip.hipStreamEndCapture(h, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None,
+                                       ctypes.c_size_t(0)) == 0
+        assert hip.hipGraphLaunch(exe, h) == 0
+        side.synchronize()
+        assert torch.equal(kept.cpu(), ref[0]) and torch.equal(bits(wg), bits(ref[1]))
+        assert torch.equal(bits(x["k"]), bits(ref[2])) and torch.equal(bits(x["v"]), bits(ref[3]))
+        assert hip.hipGraphExecDestroy(exe) == 0 and hip.hipGraphDestroy(graph) == 0
+
+
 def test_a_request_with_a_bad_table_is_left_alone():
     c = mr.paged([200, 100, 90], 2, 64, 16, torch.bfloat16, seed=4)
     w = weights_of(c, 2, 16, 4, "long")

@@ -261,6 +261,73 @@ def test_append_leaves_the_other_slots(dt, layout, T, held, d, ps):
     assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
 
 
+@pytest.mark.parametrize("layout", ["tokmajor", "dmajor"])
+@pytest.mark.parametrize("counts", [[1, 1, 1, 1], [3, 1200, 700, 1100]])
+@pytest.mark.parametrize("csr", [False, True])
+def test_append_skips_what_has_no_place(layout, counts, csr):
+    """Request 1 has a page outside the pool, request 2 a table that is too short (a CSR one
+    by its own list); some positions lie outside the rotation's table."""
+    dt, hq, hkv, d, ps = torch.bfloat16, 6, 2, 128, 16
+    T, R, held = sum(counts), 4, [5, 0, 20, 33]
+    g = torch.Generator().manual_seed(T)
+    qkv, qw, kw = case(T, hq, hkv, d, dt, 14)
+    need = [-(-(h + n) // ps) for h, n in zip(held, counts)]
+    have = [n - 1 if r == 2 else n for r, n in enumerate(need)]
+    P = sum(need) + 1
+    perm = torch.randperm(P, generator=g).tolist()
+    rows, at = [], 0
+    for n in have:
+        rows.append(perm[at:at + n])
+        at += n
+    rows[1][-1] = P
+    kp = torch.randn(P, hkv, ps, d, generator=g).to(dt)
+    vp = torch.randn(*((P, hkv, d, ps) if layout == "dmajor" else kp.shape), generator=g).to(dt)
+    pos = torch.randint(0, 512, (T,), generator=g)
+    pos[torch.rand(T, generator=g) < 0.2] = 512
+    pos[0] = 3
+    table = rotary.cos_sin_table(512, d)
+    app = [0]
+    for n in counts:
+        app.append(app[-1] + n)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    if csr:
+        ind = [0]
+        for r in rows:
+            ind.append(ind[-1] + len(r))
+        bt, tk = i32([p for r in rows for p in r]), dict(page_indptr=i32(ind))
+    else:
+        width = max(need)
+        bt, tk = i32([r + [-1] * (width - len(r)) for r in rows]), {}
+    x, kd, vd = qkv.cuda(), kp.cuda(), vp.cuda()
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    qo = torch.full((T, hq, d), 7.0, dtype=dt, device="cuda")
+    q = rotary.append_rotated(x[:, :hq], x[:, hq:hq + hkv], x[:, hq + hkv:], pos.cuda(), table,
+                              i32(app), i32([h + n for h, n in zip(held, counts)]), kd, vd, bt,
+                              v_layout=layout, q_weight=cu(qw), k_weight=cu(kw), errors=err,
+                              q_out=qo, **tk)
+    rq, rk = rotary.qk_norm_rope(x[:, :hq], x[:, hq:hq + hkv], pos.clamp(max=511).cuda(), table,
+                                 q_weight=cu(qw), k_weight=cu(kw))
+    rk, bad = rk.cpu(), 0
+    for r in range(R):
+        for i in range(counts[r]):
+            t, b, s = app[r] + i, (held[r] + i) // ps, (held[r] + i) % ps
+            if pos[t] == 512:
+                bad += 1
+                continue
+            if b >= len(rows[r]) or rows[r][b] == P:
+                bad += hkv
+                continue
+            kp[rows[r][b], :, s] = rk[t]
+            if layout == "dmajor":
+                vp[rows[r][b], :, :, s] = qkv[t, hq + hkv:]
+            else:
+                vp[rows[r][b], :, s] = qkv[t, hq + hkv:]
+    ok = pos < 512
+    assert torch.equal(q.cpu()[ok], rq.cpu()[ok]) and (q.cpu()[~ok] == 7).all()
+    assert torch.equal(kd.cpu(), kp) and torch.equal(vd.cpu(), vp)
+    assert int(err) == bad
+
+
 def test_append_without_a_place_is_counted():
     hq, hkv, d, ps = 2, 3, 64, 16
     qkv, qw, kw = case(20, hq, hkv, d, torch.bfloat16, 10)
