@@ -19,10 +19,13 @@
 //
 // fp32 caches keep fp32 all the way, through the fp32 matrix instruction (4 dims, or 4
 // tokens, a step): a lane's 16 bytes of a key row are its dims of four steps, the lane's four
-// probabilities the tokens 4 (lane / 16) + t of step t. 8 flops a byte, a third of the rate
-// at which those bytes arrive.
+// probabilities the tokens 4 (lane / 16) + t of step t. Its 8 flops a byte are 50 TFLOP/s
+// at the rate of the bytes, a third of what that instruction does.
 //
-// Bound by the cache's bytes.
+// Bound by the cache's bytes. Measured: 64 requests of 2048 tokens, 32 / 8 heads of 128, bf16,
+// weighted 87 us (6.3 TB/s; the plain decode 83); 48 of 200..2900, differential, 62 us (4.9);
+// fp32, 64 of 1000 tokens, 3 kv-heads, differential 36 us (5.4); one request of 100003 in 64
+// chunks 69 us (6.0), then 7 us of join.
 #pragma once
 
 #include "decode_mfma.h"
