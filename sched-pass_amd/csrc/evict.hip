@@ -15,7 +15,7 @@
 //   fp8: a third launch stores the pages' new scales, behind the last read of the old ones.
 // Bound by the moved bytes, and for few tasks by the launches behind each other. Measured,
 // bf16, 8 kv-heads of 128: 32 requests of 2048, half kept, 78 us (selection 18, moves 60: 4.5
-// TB/s); one of 65537, an eighth kept, 84 us (selection 53 in six launches, moves 28).
+// TB/s); one of 65537, an eighth kept, 63 us (selection 35 in six launches, moves 28).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -427,7 +427,10 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
 // wide_digit launches count the digits [31:21], [20:10] and [9:0] of the keys, each among those
 // that agree with the digits before; wide_count counts each chunk's kept tokens and ties;
 // wide_keep writes them. Weights move with the rows, in evict_move's grid.
-constexpr int kWide = 256, kWideReg = 16;
+// (Tokens of a workgroup, in us for one request of 65537 with 8 kv-heads, two of 25820 with 2,
+// 14 of 30000 with 8: 4096 83.9 / 70.0 / 159, 2048 in 256 lanes 71.7 / 57.9 / 151, in 512 62.4 /
+// 51.1 / 160, 1024 63.7 / 48.0 / 187.)
+constexpr int kWide = 512, kWideReg = 4;
 constexpr uint32_t kWideSpan = kWide * kWideReg, kWideBins = 2048;
 
 __device__ __forceinline__ uint32_t *wide_hist(const EParams &P, uint32_t task) {
@@ -1065,7 +1068,7 @@ uint32_t new_pages_of(const SchedEvictArgs *a) {
 
 // Tables that reach past one workgroup's registers (evict_select<512, 24>'s 12288 tokens),
 // of fewer tasks than half the compute units, take the wide selection: 8 tasks of 65537
-// tokens 198 -> 93 us with the moves, 4 of 25820 119 -> 98; 8 of 16310, which fit, 47 -> 67.
+// tokens 198 -> 63 us with the moves, 4 of 25820 119 -> 51; 8 of 12000, which fit, 46 -> 51.
 constexpr uint32_t kWideTasks = 128, kShort = 256u * 16u, kOneRead = 512u * 24u;
 
 bool wide_applies(const SchedEvictArgs *a) {
