@@ -15,7 +15,7 @@
 //   fp8: a third launch stores the pages' new scales, behind the last read of the old ones.
 // Bound by the moved bytes, and for few tasks by the launches behind each other. Measured,
 // bf16, 8 kv-heads of 128: 32 requests of 2048, half kept, 78 us (selection 18, moves 60: 4.5
-// TB/s); one of 65537, an eighth kept, 63 us (selection 35 in six launches, moves 28).
+// TB/s); one of 65537, an eighth kept, 51 us (selection 34 in six launches, moves 16).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -45,10 +45,12 @@ struct EParams {
   uint32_t sink, recent;
   uint32_t num_pages;
   uint32_t ps_magic; // ceil(2^32 / ps): t / ps for t up to 2^24
-  uint32_t row_groups; // evict_move: workgroups that move rows (then weights, a task each)
+  uint32_t row_groups; // evict_move: workgroups that move rows (then those of saved weights)
   // the wide selection: per task three histograms, whether its table is bad, and per chunk
   // its kept tokens and ties
   uint32_t *wide, chunks;
+  float *saved; // the wide selection's kept weights, [task][most_kept]
+  uint32_t most_kept, save_chunks;
   // evict_move_few: per task and tensor a ticket and a flag for each of its chunks
   uint32_t *moves, move_chunks;
 };
@@ -160,15 +162,16 @@ __device__ __forceinline__ void pick_digit(const uint32_t (*s_hist)[256], uint32
 // The kept tokens of a stretch in order: NT lanes with KREG tokens each, x their weights (token
 // t0 + i NT + lane). Those outside [lo, hi) stay, of the others those whose key is above T
 // and the first `left` of key T; *base and *seen are the kept tokens and the ties before
-// the stretch, and go on. WEIGHTS: their weights move along (in place: every lane has the
+// the stretch, and go on. Their weights go to `saved`, or with WEIGHTS move along (in place: every lane has the
 // stretch's before one is overwritten, and those of later stretches lie behind every slot
 // that is written here).
 template <int NT, int KREG, bool WEIGHTS>
 __device__ __forceinline__ void keep_stretch(const EParams &P, const Req &q, uint32_t h,
                                              const float (&x)[KREG], uint32_t t0, uint32_t lo,
                                              uint32_t hi, uint32_t want, uint32_t T,
-                                             uint32_t left, int32_t *kept, uint32_t *s_cnt,
-                                             uint32_t *s_wave, uint32_t *base, uint32_t *seen) {
+                                             uint32_t left, int32_t *kept, float *saved,
+                                             uint32_t *s_cnt, uint32_t *s_wave, uint32_t *base,
+                                             uint32_t *seen) {
   constexpr uint32_t NW = NT / 64;
   constexpr uint32_t E = (KREG * NW + NT - 1) / NT; // counts of a lane in a scan
   static_assert(KREG <= 32, "a bit for each token of a lane");
@@ -244,6 +247,8 @@ __device__ __forceinline__ void keep_stretch(const EParams &P, const Req &q, uin
     const uint32_t at = *base + s_cnt[i * NW + wave] + (uint32_t)__popcll(b & below);
     if (in && at < q.m) {
       kept[at] = (int32_t)t;
+      if (!WEIGHTS)
+        saved[at] = x[i];
       if (WEIGHTS && (t != at || P.wo != P.w)) {
         const uint32_t d = div_ps(P, at);
         P.wo[(int64_t)P.bt[q.row + d] * P.w_ps + (int64_t)h * P.w_hs + (at - d * P.ps)] = x[i];
@@ -410,8 +415,8 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
   for (uint32_t t0 = 0; t0 < q.n; t0 += SPAN) {
     if (!one)
       load(t0);
-    keep_stretch<NT, KREG, true>(P, q, h, x, t0, lo, hi, want, T, left, kept, s_cnt, s_wave, &base,
-                                 &seen);
+    keep_stretch<NT, KREG, true>(P, q, h, x, t0, lo, hi, want, T, left, kept, nullptr, s_cnt, s_wave,
+                                 &base, &seen);
   }
   for (uint32_t j = q.m + tid; j < P.max_keep; j += NT)
     kept[j] = -1;
@@ -426,7 +431,8 @@ template <int NT, int KREG> __global__ void __launch_bounds__(NT) evict_select(E
 // The same selection in steps: wide_start checks the table and clears the histograms; three
 // wide_digit launches count the digits [31:21], [20:10] and [9:0] of the keys, each among those
 // that agree with the digits before; wide_count counts each chunk's kept tokens and ties;
-// wide_keep writes them. Weights move with the rows, in evict_move's grid.
+// wide_keep writes them and saves their weights, which go to their slots beside the rows, in
+// evict_move's grid.
 // (Tokens of a workgroup, in us for one request of 65537 with 8 kv-heads, two of 25820 with 2,
 // 14 of 30000 with 8: 4096 83.9 / 70.0 / 159, 2048 in 256 lanes 71.7 / 57.9 / 151, in 512 62.4 /
 // 51.1 / 160, 1024 63.7 / 48.0 / 187.)
@@ -605,7 +611,8 @@ __global__ void __launch_bounds__(kWide) wide_keep(EParams P) {
     base = t0;
   }
   keep_stretch<kWide, kWideReg, false>(P, c.q, c.h, x, t0, c.lo, c.hi, c.want, T, left,
-                                       P.kept + (int64_t)c.task * P.max_keep, s_cnt, s_wave, &base,
+                                       P.kept + (int64_t)c.task * P.max_keep,
+                                       P.saved + (int64_t)c.task * P.most_kept, s_cnt, s_wave, &base,
                                        &seen);
 }
 
@@ -656,35 +663,22 @@ template <typename U> __device__ __forceinline__ void recode(U &, float) {}
 constexpr int kMove = 512;
 constexpr uint32_t kStage = 2048; // rows whose places are in LDS at a time
 
-// A task's weights after the wide selection, by one workgroup: as the rows below, a round of
-// kMove * 8 weights read before it is written.
-__device__ __forceinline__ void move_weights(const EParams &P, uint32_t task) {
-  constexpr int N = 8;
+// Saved weights to their slots: chunk `which` % save_chunks of a task. (Gathered from their old
+// slots by one workgroup a task, a round read before it is written, the 50000 kept weights
+// of one request of 100000 took 69 us more.)
+constexpr uint32_t kSaved = kMove * 8;
+
+__device__ __forceinline__ void put_weights(const EParams &P, uint32_t which) {
+  const uint32_t task = which / P.save_chunks, j0 = which % P.save_chunks * kSaved;
   const uint32_t r = task / P.Hkv, h = task % P.Hkv;
   const Req q = req_of(P, r);
-  const int32_t *kept = P.kept + (int64_t)task * P.max_keep;
-  if (q.m == 0u || kept[0] < 0 || (q.m == q.n && P.wo == P.w))
+  if (j0 >= q.m || P.kept[(int64_t)task * P.max_keep] < 0 || (q.m == q.n && P.wo == P.w))
     return;
-  for (uint32_t j0 = 0; j0 < q.m; j0 += kMove * N) {
-    float x[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t j = j0 + (uint32_t)i * kMove + threadIdx.x;
-      if (j < q.m) {
-        const uint32_t t = (uint32_t)kept[j], b = div_ps(P, t);
-        x[i] = P.w[(int64_t)P.bt[q.row + b] * P.w_ps + (int64_t)h * P.w_hs + (t - b * P.ps)];
-      }
-    }
-    __builtin_amdgcn_s_waitcnt(kVmcnt0);
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const uint32_t j = j0 + (uint32_t)i * kMove + threadIdx.x;
-      if (j < q.m) {
-        const uint32_t b = div_ps(P, j);
-        P.wo[(int64_t)P.bt[q.row + b] * P.w_ps + (int64_t)h * P.w_hs + (j - b * P.ps)] = x[i];
-      }
-    }
+  const float *saved = P.saved + (int64_t)task * P.most_kept;
+  const uint32_t end = min(q.m, j0 + kSaved);
+  for (uint32_t j = j0 + threadIdx.x; j < end; j += kMove) {
+    const uint32_t b = div_ps(P, j);
+    P.wo[(int64_t)P.bt[q.row + b] * P.w_ps + (int64_t)h * P.w_hs + (j - b * P.ps)] = saved[j];
   }
 }
 
@@ -889,7 +883,7 @@ __global__ void __launch_bounds__(kMove, 4) evict_move(EParams P, Mode k_mode, M
   __shared__ int64_t s_from[kStage], s_to[kStage];
   __shared__ float s_ratio[FP8 ? kStage : 1];
   if (blockIdx.x >= P.row_groups) { // the wide selection's weights
-    move_weights(P, blockIdx.x - P.row_groups);
+    put_weights(P, blockIdx.x - P.row_groups);
     return;
   }
   const uint32_t task = blockIdx.x >> 1;
@@ -920,23 +914,28 @@ __global__ void __launch_bounds__(kMove, 4) evict_move(EParams P, Mode k_mode, M
 // once all chunks before it have said so: what it overwrites are tokens of theirs or its own.
 // A chunk waits for earlier tickets only, whose workgroups are running and wait for nothing
 // before they say so; every wait ends.
-constexpr int kFewUnits = 8; // 16-byte units of a lane
+//
+// 16-byte units of a lane, 8 and 4: one request of 65537 tokens, an eighth kept, 51 / 55 us, 4
+// of 8000 55 / 59; with d-major values 2 of 2000 33 / 26, 64 of 1000 fp8 143 / 128, one of 65537
+// 88 / 91.
+__host__ __device__ constexpr int few_units(bool turned) { return turned ? 4 : 8; }
 
 // Tokens of a chunk: a multiple of 16, so that a turned unit lies in one chunk.
-__host__ __device__ inline uint32_t few_rows(uint32_t units) {
-  return kMove / units * kFewUnits & ~15u;
+__host__ __device__ inline uint32_t few_rows(uint32_t units, bool turned) {
+  return kMove / units * few_units(turned) & ~15u;
 }
 
 template <int EB, bool TURNED>
 __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
   constexpr bool FP8 = EB == 1;
-  constexpr uint32_t MOST = kMove / 4 * kFewUnits; // tokens of a chunk (4 units each at least)
+  constexpr int UNITS = few_units(TURNED);
+  constexpr uint32_t MOST = kMove / 4 * UNITS; // tokens of a chunk (4 units each at least)
   constexpr uint32_t TOK = 16 / EB;
   __shared__ int64_t s_from[MOST], s_to[MOST];
   __shared__ float s_ratio[FP8 ? MOST : 1];
   __shared__ uint32_t s_chunk;
   if (blockIdx.x >= P.row_groups) { // the wide selection's weights
-    move_weights(P, blockIdx.x - P.row_groups);
+    put_weights(P, blockIdx.x - P.row_groups);
     return;
   }
   const uint32_t tid = threadIdx.x, which = blockIdx.x % (2u * P.R * P.Hkv), task = which >> 1;
@@ -950,7 +949,7 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
   if (tid == 0)
     s_chunk = atomicAdd(ticket, 1u);
   __syncthreads();
-  const uint32_t units = P.D * EB / 16u, each = few_rows(units), chunk = s_chunk;
+  const uint32_t units = P.D * EB / 16u, each = few_rows(units, TURNED), chunk = s_chunk;
   const uint32_t j0 = chunk * each;
   if (j0 >= q.m)
     return;
@@ -962,11 +961,11 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
   const bool turned = TURNED && vals;
   const uint32_t most = (cnt + TOK - 1u) / TOK * P.D;
   const uint32_t rows = kMove / units, rr = tid / units, off = tid % units * 16u;
-  uint4 x[kFewUnits];
+  uint4 x[UNITS];
   uint32_t moves = 0u;
   if (!turned) {
 #pragma unroll
-    for (int i = 0; i < kFewUnits; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
       const uint32_t k = (uint32_t)i * rows + rr;
       x[i] = uint4{};
       if (rr < rows && k < cnt && s_from[k] >= 0) {
@@ -976,7 +975,7 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < kFewUnits; ++i) {
+    for (int i = 0; i < UNITS; ++i) {
       const uint32_t p = (uint32_t)i * kMove + tid, pc = min(p, most - 1u);
       const bool any =
           gather16<EB>(S.pool + pc % P.D * S.dim, s_from, pc / P.D * TOK, cnt, x[i]);
@@ -985,7 +984,7 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
     }
   }
 #pragma unroll
-  for (int i = 0; i < kFewUnits; ++i)
+  for (int i = 0; i < UNITS; ++i)
     hold(x[i]);
   __builtin_amdgcn_s_waitcnt(kVmcnt0);
   __syncthreads(); // the chunk is in registers: nothing to publish but that
@@ -997,7 +996,7 @@ __global__ void __launch_bounds__(kMove) evict_move_few(EParams P) {
         __builtin_amdgcn_s_sleep(1);
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kFewUnits; ++i) {
+  for (int i = 0; i < UNITS; ++i) {
     if (!((moves >> i) & 1u))
       continue;
     if (turned) {
@@ -1068,7 +1067,7 @@ uint32_t new_pages_of(const SchedEvictArgs *a) {
 
 // Tables that reach past one workgroup's registers (evict_select<512, 24>'s 12288 tokens),
 // of fewer tasks than half the compute units, take the wide selection: 8 tasks of 65537
-// tokens 198 -> 63 us with the moves, 4 of 25820 119 -> 51; 8 of 12000, which fit, 46 -> 51.
+// tokens 198 -> 51 us with the moves, 4 of 25820 119 -> 44; 8 of 12000, which fit, 46 -> 51.
 constexpr uint32_t kWideTasks = 128, kShort = 256u * 16u, kOneRead = 512u * 24u;
 
 bool wide_applies(const SchedEvictArgs *a) {
@@ -1088,7 +1087,7 @@ uint64_t wide_bytes(const SchedEvictArgs *a) {
   if (!wide_applies(a))
     return 0;
   const uint64_t tasks = (uint64_t)a->num_requests * a->num_kv_heads;
-  return tasks * (3u * kWideBins + 1u + 2u * wide_chunks(a)) * 4u;
+  return tasks * (3u * kWideBins + 1u + 2u * wide_chunks(a) + most_kept(a)) * 4u;
 }
 // Each tensor in 16-byte units where its strides allow. d-major, 8 kv-heads of 128 (us, V by
 // element / turned): 32 requests of 2048, half kept, 258 / 160; 2 of 2000 168 / 33; one of
@@ -1123,7 +1122,8 @@ bool few_applies(const SchedEvictArgs *a) {
 }
 uint32_t few_chunks(const SchedEvictArgs *a) {
   const uint32_t units = a->head_dim * elem_bytes(a->kv_dtype) / 16u;
-  return (most_kept(a) + few_rows(units) - 1u) / few_rows(units);
+  const uint32_t rows = few_rows(units, a->v_dim_stride != 1);
+  return (most_kept(a) + rows - 1u) / rows;
 }
 uint64_t move_bytes(const SchedEvictArgs *a) {
   if (!few_applies(a))
@@ -1210,6 +1210,9 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   if (many) {
     P.wide = reinterpret_cast<uint32_t *>(static_cast<uint8_t *>(a->workspace) + scale_bytes(a));
     P.chunks = wide_chunks(a);
+    P.most_kept = most_kept(a), P.save_chunks = (P.most_kept + kSaved - 1u) / kSaved;
+    P.saved = reinterpret_cast<float *>(P.wide + (uint64_t)tasks * (3u * kWideBins + 1u +
+                                                                   2u * P.chunks));
     const dim3 grid(tasks, P.chunks);
     hipLaunchKernelGGL(wide_start, dim3(tasks), dim3(kWide), 0, s, P);
     for (int digit = 0; digit < 3; ++digit)
@@ -1227,7 +1230,7 @@ int sched_kv_evict(const SchedEvictArgs *a, void *stream) {
   hipError_t e = hipGetLastError();
   if (e == hipSuccess && a->max_keep > 0) {
     P.row_groups = 2u * tasks * (few ? P.move_chunks : 1u);
-    const dim3 grid(P.row_groups + (many ? tasks : 0u)), block(kMove);
+    const dim3 grid(P.row_groups + (many ? tasks * P.save_chunks : 0u)), block(kMove);
     if (few) {
       const bool turned = v_mode == kTurned;
       auto fn = eb == 1   ? (turned ? evict_move_few<1, true> : evict_move_few<1, false>)
